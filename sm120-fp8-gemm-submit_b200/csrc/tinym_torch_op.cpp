@@ -26,10 +26,15 @@
 #include <torch/library.h>
 
 #include <cmath>
+#include <string>
 
 #include "../../include/tinym_b200.h"
 
 namespace {
+
+// Numbers go into messages as text: formatting them through the message's
+// stream crashes where the compiler's libstdc++ is not the one loaded.
+std::string num(int64_t v) { return std::to_string(v); }
 
 void check_inputs(const at::Tensor& a, const at::Tensor& b) {
     TORCH_CHECK(a.is_cuda() && b.is_cuda(), "A and B must be CUDA tensors");
@@ -115,8 +120,8 @@ at::Tensor run_packed(const at::Tensor& a, const at::Tensor& bp, int64_t n, int6
                 "B_packed must be the uint8 tensor returned by pack_weights");
     int64_t bytes = 0;
     raise_status(tinym_packed_weight_bytes(n, k, &bytes));
-    TORCH_CHECK(bp.numel() == bytes, "B_packed has ", bp.numel(), " bytes, packed [", n, ", ",
-                k, "] needs ", bytes);
+    TORCH_CHECK(bp.numel() == bytes, "B_packed has ", num(bp.numel()), " bytes, packed [", num(n),
+                ", ", num(k), "] needs ", num(bytes));
     TORCH_CHECK(alpha.is_cuda() && alpha.scalar_type() == at::ScalarType::Float &&
                     alpha.numel() == 1,
                 "alpha must be a one-element CUDA float32 tensor");
