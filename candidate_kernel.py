@@ -31,6 +31,10 @@ Differences from the reference adapter:
   (BF16 or FP32): the per-tensor E4M3 quantisation of the harness's
   ``quantize_per_tensor`` (fp8_gemm_task_harness.py:41-44) runs on the device
   as a prologue overlapped with the GEMM's weight stream.
+* operators the reference has no counterpart of: ``fp8_gemm_grouped`` (any
+  number of rows sorted by expert, one weight per expert) and MXFP4 --
+  ``mxfp4_quantize``, ``mxfp4_dequantize``, ``mxfp4_gemm``,
+  ``mxfp4_gemm_grouped``.
 
 There is no fallback: if the native library cannot be loaded, ``build()``
 raises.
@@ -158,6 +162,73 @@ def fp8_gemm_act(x: torch.Tensor, b: torch.Tensor, w_scale: torch.Tensor):
     if not _BUILT:
         build()
     return _run_quant_act(x, b, w_scale)
+
+
+def fp8_gemm_grouped(a: torch.Tensor, b: torch.Tensor, alpha: torch.Tensor, offsets: torch.Tensor,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """One weight per group of rows (mixture of experts): row r of the result is
+    bf16(alpha[e] * (a[r].float() @ b[e].float().T)) for the expert e with
+    offsets[e] <= r < offsets[e + 1].
+
+    a [rows, K] E4M3 holds the rows sorted by expert, b [experts, N, K] E4M3,
+    alpha one float32 value or one per expert, offsets [experts + 1] int32,
+    non-decreasing.  Everything stays on the device: the group sizes are read
+    there, so a captured call replays with other groups, and alpha is used
+    without a check.  Rows of no expert are zeros, or left as they were in
+    `out` ([rows, N] BF16, unit column stride)."""
+    if not _BUILT:
+        build()
+    if out is None:
+        return torch.ops.sm120_fp8_gemm.run_grouped(a, b, alpha, offsets)
+    torch.ops.sm120_fp8_gemm.run_grouped_out(a, b, alpha, offsets, out)
+    return out
+
+
+def mxfp4_quantize(x: torch.Tensor):
+    """x [rows, K] or [batch, rows, K] (BF16 / FP32, K % 32 == 0) as MXFP4:
+    (codes, scales).  codes uint8 [.., rows, K / 2], the even column in the low
+    nibble; scales uint8 [.., ceil(rows / 128), ceil(K / 128), 512], the block
+    order described in include/tinym_b200.h.  The scale of 32 columns is
+    2^(floor(log2(amax)) - 2), the elements are rounded to nearest even and
+    saturated; a block that holds a NaN or an infinity becomes NaN."""
+    if not _BUILT:
+        build()
+    return torch.ops.sm120_fp8_gemm.mxfp4_quantize(x)
+
+
+def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
+                     dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The values of mxfp4_quantize's result, in BF16 or FP32 (exact)."""
+    if not _BUILT:
+        build()
+    return torch.ops.sm120_fp8_gemm.mxfp4_dequantize(codes, scales, dtype)
+
+
+def mxfp4_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
+               alpha: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """bf16(alpha * a @ b.T) of two MXFP4 matrices a [M, K] and b [N, K] (codes
+    and scales of mxfp4_quantize), FP32 accumulation.  alpha: one float32 CUDA
+    value, 1 by default."""
+    if not _BUILT:
+        build()
+    if out is None:
+        return torch.ops.sm120_fp8_gemm.run_mxfp4(a, a_scales, b, b_scales, alpha)
+    torch.ops.sm120_fp8_gemm.run_mxfp4_out(a, a_scales, b, b_scales, alpha, out)
+    return out
+
+
+def mxfp4_gemm_grouped(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor,
+                       b_scales: torch.Tensor, offsets: torch.Tensor,
+                       alpha: torch.Tensor | None = None,
+                       out: torch.Tensor | None = None) -> torch.Tensor:
+    """fp8_gemm_grouped with MXFP4 operands: a [rows, K] sorted by expert and
+    b [experts, N, K] as codes and scales of mxfp4_quantize."""
+    if not _BUILT:
+        build()
+    if out is None:
+        return torch.ops.sm120_fp8_gemm.run_mxfp4_grouped(a, a_scales, b, b_scales, offsets, alpha)
+    torch.ops.sm120_fp8_gemm.run_mxfp4_grouped_out(a, a_scales, b, b_scales, offsets, alpha, out)
+    return out
 
 
 __all__ = ["build", "prepare_weights", "fp8_gemm"]

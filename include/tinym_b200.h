@@ -298,6 +298,77 @@ TINYM_API int tinym_ipc_export(const void* ptr, void* handle, int64_t* offset);
 TINYM_API int tinym_ipc_open(const void* handle, void** base);
 TINYM_API int tinym_ipc_close(void* base);
 
+/* ------------------------------------------------------------------------
+ * Grouped products: one weight per group of rows (mixture of experts)
+ *
+ *   Y[r, n] = bf16( alpha[e] * sum_k X[r, k] * W[e, n, k] ),
+ *                                offsets[e] <= r < offsets[e + 1]
+ *
+ * X [rows, K] holds the rows sorted by expert, W [experts, N, K] one weight
+ * per expert, offsets_dev experts + 1 non-decreasing int32 row numbers on the
+ * device (NULL: one expert, all rows).  They are read on the device when the
+ * kernel runs, so a captured graph replays with other groups.  Offsets
+ * outside [0, rows] are clamped to it and an offset below an earlier one is
+ * raised to that one, so that no offsets reach memory outside X and Y.
+ * An expert may have no rows; a row before offsets[0] or from
+ * offsets[experts] on belongs to none: it is left as it was, or written as
+ * zeros under TINYM_FLAG_ZERO_REST.
+ *
+ * alpha_dev: alpha_count = 1 value for all experts, or `experts` values; NULL
+ * means 1.  It is used as it is (a non-finite alpha gives non-finite rows).
+ * Any number of rows >= 1 and any N; K % 16 == 0; up to 1024 experts.  Sums
+ * are FP32 over the whole of K in one fixed order: a row's result depends
+ * neither on the run nor on the split of the work over SMs.
+ */
+#define TINYM_FLAG_ZERO_REST 2u
+TINYM_API int tinym_fp8_gemm_grouped(const void* x, const void* w, void* y, int64_t ldy,
+                                     int64_t rows, int64_t experts, int64_t n, int64_t k,
+                                     const int32_t* offsets_dev, const float* alpha_dev,
+                                     int32_t alpha_count, uint32_t flags, void* stream);
+
+/* ------------------------------------------------------------------------
+ * MXFP4: E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), one
+ * E8M0 scale byte s (2^(s - 127); 255 = NaN) per 32 consecutive columns.
+ *
+ * Codes: [rows, K / 2] bytes, the even column in the low nibble; K % 32 == 0.
+ * Scales: blocks of 128 rows x 4 scales (128 columns), 512 bytes each, laid
+ * out [ceil(rows / 128)][ceil(K / 128)][512]; scale c of row r is byte
+ *   16 (r % 32) + 4 (r / 32 % 4) + c % 4   of block [r / 128][c / 4],
+ * the order that the tensor core's scale copy takes.  Bytes past the rows or
+ * past K are padding: written as zeros, never used.  A batch of matrices
+ * (expert weights) repeats both layouts.
+ */
+
+/* Scale bytes of `batch` [rows, K] matrices. */
+TINYM_API int tinym_mxfp4_scale_bytes(int64_t batch, int64_t rows, int64_t k, int64_t* bytes);
+
+/* Quantise x [batch, rows, K] (dtype TINYM_ACT_BF16 / TINYM_ACT_F32): per
+ * block scale 2^e with e = floor(log2(amax)) - 2 clamped to [-127, 127],
+ * elements rounded to nearest even and saturated at 6.  A block that holds a
+ * NaN or an infinity gets scale 255 and zero codes. */
+TINYM_API int tinym_mxfp4_quantize(const void* x, int32_t dtype, void* codes, void* scales,
+                                   int64_t batch, int64_t rows, int64_t k, void* stream);
+
+/* The values of codes and scales, [batch, rows, K] in dtype.  Exact, but for
+ * scales near the ends of the range, whose values overflow to infinity. */
+TINYM_API int tinym_mxfp4_dequantize(const void* codes, const void* scales, void* y, int32_t dtype,
+                                     int64_t batch, int64_t rows, int64_t k, void* stream);
+
+/* Y [M, N] = bf16( alpha * X . W^T ), both operands MXFP4 (X [M, K], W [N, K]),
+ * FP32 accumulation; alpha_dev one value or NULL (1).  Any M, N >= 1,
+ * K % 32 == 0. */
+TINYM_API int tinym_mxfp4_gemm(const void* x, const void* x_scales, const void* w,
+                               const void* w_scales, void* y, int64_t ldy, int64_t m, int64_t n,
+                               int64_t k, const float* alpha_dev, void* stream);
+
+/* The grouped product with MXFP4 operands: X [rows, K], W [experts, N, K]
+ * (one scale layout per expert); the rest as in tinym_fp8_gemm_grouped. */
+TINYM_API int tinym_mxfp4_gemm_grouped(const void* x, const void* x_scales, const void* w,
+                                       const void* w_scales, void* y, int64_t ldy, int64_t rows,
+                                       int64_t experts, int64_t n, int64_t k,
+                                       const int32_t* offsets_dev, const float* alpha_dev,
+                                       int32_t alpha_count, uint32_t flags, void* stream);
+
 /* Human-readable name of a tinym_status code (static string). */
 TINYM_API const char* tinym_status_string(int32_t status);
 

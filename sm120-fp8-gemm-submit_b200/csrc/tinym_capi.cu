@@ -29,6 +29,8 @@
 #include "../../include/tinym_b200.h"
 #include "tinym_kernels.cuh"
 #include "tinym_quant.cuh"
+#include "tinym_grouped.cuh"
+#include "tinym_mxfp4.cuh"
 
 namespace {
 
@@ -1080,3 +1082,5 @@ int tinym_pending_errors(uint32_t* flags, int32_t clear) {
 }
 
 }  // extern "C"
+
+#include "tinym_grouped_host.inl"

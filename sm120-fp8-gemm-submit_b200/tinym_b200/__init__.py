@@ -65,6 +65,12 @@ EXPORTED = (
     "tinym_ipc_export",
     "tinym_ipc_open",
     "tinym_ipc_close",
+    "tinym_fp8_gemm_grouped",
+    "tinym_mxfp4_scale_bytes",
+    "tinym_mxfp4_quantize",
+    "tinym_mxfp4_dequantize",
+    "tinym_mxfp4_gemm",
+    "tinym_mxfp4_gemm_grouped",
     "tinym_status_string",
     "tinym_last_error",
     "tinym_abi_version",
@@ -189,6 +195,21 @@ def capi() -> ctypes.CDLL:
             lib.tinym_ipc_open.restype = ctypes.c_int
             lib.tinym_ipc_close.argtypes = [vp]
             lib.tinym_ipc_close.restype = ctypes.c_int
+            i32 = ctypes.c_int32
+            lib.tinym_fp8_gemm_grouped.argtypes = [vp, vp, vp, i64, i64, i64, i64, i64, vp, vp,
+                                                   i32, ctypes.c_uint32, vp]
+            lib.tinym_fp8_gemm_grouped.restype = ctypes.c_int
+            lib.tinym_mxfp4_scale_bytes.argtypes = [i64, i64, i64, ctypes.POINTER(i64)]
+            lib.tinym_mxfp4_scale_bytes.restype = ctypes.c_int
+            lib.tinym_mxfp4_quantize.argtypes = [vp, i32, vp, vp, i64, i64, i64, vp]
+            lib.tinym_mxfp4_quantize.restype = ctypes.c_int
+            lib.tinym_mxfp4_dequantize.argtypes = [vp, vp, vp, i32, i64, i64, i64, vp]
+            lib.tinym_mxfp4_dequantize.restype = ctypes.c_int
+            lib.tinym_mxfp4_gemm.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, vp, vp]
+            lib.tinym_mxfp4_gemm.restype = ctypes.c_int
+            lib.tinym_mxfp4_gemm_grouped.argtypes = [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64,
+                                                     vp, vp, i32, ctypes.c_uint32, vp]
+            lib.tinym_mxfp4_gemm_grouped.restype = ctypes.c_int
             lib.tinym_status_string.argtypes = [ctypes.c_int32]
             lib.tinym_status_string.restype = ctypes.c_char_p
             lib.tinym_last_error.argtypes = []
