@@ -16,19 +16,32 @@
 // groups' row tiles in shared memory and every role of the CTA walks the same
 // list of pieces (group, row tile, W rows).
 //
-//  * Stream pieces (TILE = false), for few rows per group, where the time is
+//  * Stream pieces (PAIR = false), for few rows per group, where the time is
 //    W's bytes: the W rows of all non-empty groups are laid end to end in
 //    units of 8 rows and each CTA takes an equal, contiguous share of them,
 //    walked in pieces of at most 128 rows with the whole of K.  The shares
 //    differ by at most one unit, so every SM streams the same number of bytes
 //    whatever the groups are, with no split of K, no workspace and one fixed
-//    order of every sum.  A stage is 512 bytes of K, fetched by one
-//    {128 B, 8 rows, 4 chunks} box per unit.
-//  * Tile pieces (TILE = true), for many rows per group, where the time is
-//    the tensor core's: 128 W rows x up to TN X rows, 128 bytes of K a stage.
+//    order of every sum.  A stage is 512 bytes of K.
+//  * Pair pieces (PAIR = true), for many rows per group, where the time is the
+//    tensor core's: two CTAs (cta_group::2) compute 256 W rows x up to 256 X
+//    rows, 128 bytes of K a stage.  Each loads its 128 W rows and half of the
+//    X rows, so a CTA moves 256 rows of K for 128 x 256 sums where one CTA
+//    alone would move 384: the L2 feeds the SMs at ~42 bytes/clk/SM here,
+//    which held single-CTA 128 x 256 tiles at 1.77 PFLOP/s of E4M3.
 //
-// Rows of a piece past its W or X rows hold whatever the ring held before:
-// the MMA computes lanes and columns for them that nobody reads.
+// MXFP4 scales reach TMEM by tcgen05.cp in blocks of 128 rows x 4 scales
+// (lane i, column j = row 32 j + i), the order in which they lie in memory.
+// W row r is therefore always MMA row r % 128: a stream piece never crosses a
+// multiple of 128 rows, and its block is copied as it is.  X tiles start at
+// any row; their scale words are gathered into the block order.
+//
+// A stage's W and X are one box each, [chunks of 128 B][rows][128 B]: a bulk
+// copy costs its issuing thread ~90 cycles whatever its size (measured), so
+// there is a tensor map for every height that a piece can have.  The MMA reads
+// 128 W rows and whole columns of 16 whatever the piece holds: the lanes and
+// columns of rows that are not the piece's come from whatever lies there and
+// nobody reads them.
 #pragma once
 
 #include <algorithm>
@@ -37,10 +50,12 @@
 
 namespace tinym {
 
-constexpr int kGrpThreads = 256;     // warp 0 TMA, 1 MMA, 2-3 scale factors, 4-7 epilogue
+constexpr int kGrpThreads = 256;     // warp 0 TMA, 1 MMA, 2-3 scales, 4-7 epilogue
 constexpr int kGrpMaxExperts = 1024;
 constexpr int kGrpBand = 8;          // row tiles walked together for each W tile (L2 reuse)
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
+constexpr int kGrpBars = 7;          // barriers beside the two per stage
+constexpr int kSfDepth = 4;          // scale copies of a warp in flight, in stages
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
 struct GroupedParams {
@@ -55,41 +70,53 @@ struct GroupedParams {
     int32_t k_bytes;          // bytes of one operand row
     int32_t alpha_stride;     // 0: one alpha for all groups
     int32_t tn;               // X rows per tile, at most
-    int32_t units;            // stream: units of 8 W rows; tile: tiles of 128 W rows
+    int32_t units;            // per X tile; stream: units of 8 W rows, or parts; pair: 256-row tiles
+    int32_t part_units;       // stream: if non-zero, a block of 16 units is cut into parts of so many
     int32_t piece_units;      // stream: units per piece, at most
+    int32_t blocked;          // stream: pieces stay inside 128-row blocks (MXFP4)
     int32_t stages;
     int32_t chunked;          // stream: one box per unit covers the whole stage
     int32_t w_stage, x_stage, sf_stage;  // bytes
-    uint32_t bar_off, sf_off, tab_off;   // shared-memory offsets
+    uint32_t w_off, sf_off, bar_off, tab_off;  // shared-memory offsets (X ring at 0)
     uint32_t tmem_cols, acc_cols, sf_col;
     uint32_t flags;
     uint32_t* err_host;
     uint64_t timeout_ns;
 };
+// Tensor maps: W in boxes of 8 (i + 1) rows, X in boxes of four heights.
+struct GroupedMaps {
+    CUtensorMap w[kTileRows / 8];
+    CUtensorMap x[4];
+};
+__host__ __device__ constexpr int grouped_x_box(bool pair, int i) { return (pair ? 16 : 8) << i; }
 constexpr uint32_t kGrpZeroRest = 1u;  // rows of no group are written as zeros
 
+constexpr int kBlockUnits = kTileRows / 8;  // 8-row units of a 128-row block
+
 // 128-row scale blocks of the X rows of a tile: stream tiles have at most 128 rows.
-__host__ __device__ constexpr int grouped_x_scale_blocks(bool tile) { return tile ? 2 : 1; }
+__host__ __device__ constexpr int grouped_x_scale_blocks(bool pair) { return pair ? 2 : 1; }
 
 struct GroupedPiece {
-    int e, row0, rows, w0, h;
+    int e, row0, rows, w0, h;  // group, X rows, W rows (pair: of both CTAs)
 };
 
 // The pieces of one CTA, in the order in which every role walks them.
-template <bool TILE>
+template <bool PAIR>
 struct GroupedWalk {
     const int32_t* off;     // [experts + 1] group starts
-    const int32_t* prefix;  // [experts + 1] row tiles before each group
-    int experts, units, piece_units, tn;
+    const int32_t* prefix;  // [experts + 1] X tiles before each group
+    int experts, n_units, units, part_units, piece_units, tn;
+    bool blocked;
     int cur, end, step;
     int e;
 
     __host__ __device__ GroupedWalk(const GroupedParams& p, const int32_t* o, const int32_t* pre,
                                     int block, int blocks)
-        : off(o), prefix(pre), experts(p.experts), units(p.units), piece_units(p.piece_units),
-          tn(p.tn), e(-1) {
+        : off(o), prefix(pre), experts(p.experts), n_units((p.n + 7) / 8), units(p.units),
+          part_units(p.part_units), piece_units(p.piece_units), tn(p.tn), blocked(p.blocked != 0),
+          e(-1) {
         const int64_t total = static_cast<int64_t>(pre[p.experts]) * p.units;
-        if constexpr (TILE) {
+        if constexpr (PAIR) {
             cur = block;
             end = static_cast<int>(total);
             step = blocks;
@@ -102,7 +129,17 @@ struct GroupedWalk {
 
     __host__ __device__ static int least(int a, int b) { return a < b ? a : b; }
 
+    // First unit of part i of a matrix.
+    __host__ __device__ int part_unit(int i) const {
+        const int per = (kBlockUnits + part_units - 1) / part_units;
+        return i / per * kBlockUnits + i % per * part_units;
+    }
+
     __host__ __device__ bool next(GroupedPiece* w) {
+        if constexpr (!PAIR) {
+            // parts past N in a matrix's last block
+            while (part_units && cur < end && part_unit(cur % units) >= n_units) ++cur;
+        }
         if (cur >= end) return false;
         const int seg = cur / units;
         if (e < 0 || seg >= prefix[e + 1]) {
@@ -117,29 +154,37 @@ struct GroupedWalk {
         const int tiles = prefix[e + 1] - prefix[e];
         const int count = off[e + 1] - off[e];
         int t;
-        if constexpr (TILE) {
+        if constexpr (PAIR) {
             const int local = cur - prefix[e] * units;
             const int band = local / (kGrpBand * units);
             const int width = least(kGrpBand, tiles - band * kGrpBand);
             const int rem = local - band * kGrpBand * units;
             const int wt = rem / width;
             t = band * kGrpBand + rem - wt * width;
-            w->w0 = wt * kTileRows;
-            w->h = kTileRows;
+            w->w0 = wt * 2 * kTileRows;
+            w->h = 2 * kTileRows;
             cur += step;
         } else {
             t = seg - prefix[e];
-            const int u = cur - seg * units;
-            const int left = least(end - cur, units - u);
-            const int pieces = (left + piece_units - 1) / piece_units;
-            const int take = (left + pieces - 1) / pieces;
+            int u = cur - seg * units, take;
+            if (part_units) {
+                u = part_unit(u);
+                take = least(least(part_units, kBlockUnits - u % kBlockUnits), n_units - u);
+                ++cur;
+            } else {
+                int left = least(end - cur, units - u);
+                if (blocked) left = least(left, kBlockUnits - u % kBlockUnits);
+                const int pieces = (left + piece_units - 1) / piece_units;
+                take = (left + pieces - 1) / pieces;
+                cur += take;
+            }
             w->w0 = u * 8;
             w->h = take * 8;
-            cur += take;
         }
-        // Equal tiles in whole MMA columns of 16: 300 rows are 160 + 140, not
-        // 256 + 44.  (tiles - 1) * wide < count, since wide <= tn.
-        const int wide = ((count + tiles - 1) / tiles + 15) & ~15;
+        // Equal tiles in whole steps of the MMA's columns: 300 rows are 160 +
+        // 140, not 256 + 44.  (tiles - 1) * wide < count, since wide <= tn.
+        constexpr int kStep = PAIR ? 32 : 16;
+        const int wide = ((count + tiles - 1) / tiles + kStep - 1) & ~(kStep - 1);
         w->e = e;
         w->row0 = off[e] + t * wide;
         w->rows = least(wide, count - t * wide);
@@ -149,7 +194,7 @@ struct GroupedWalk {
 
 // How a call is cut.
 struct GroupedPlan {
-    bool tile;
+    bool pair;
     int grid;
     uint32_t smem;
     GroupedParams prm;  // the shape and layout fields
@@ -165,51 +210,71 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     GroupedParams& p = g.prm;
     const int64_t groups = std::min(experts, rows);
     const int64_t avg = (rows + groups - 1) / groups;
-    g.tile = avg > 64;
+    g.pair = avg > 64;
     p.rows = static_cast<int32_t>(rows);
     p.experts = static_cast<int32_t>(experts);
     p.n = static_cast<int32_t>(n);
     p.k_bytes = static_cast<int32_t>(k_bytes);
     const int64_t k_chunks = (k_bytes + kBlockK - 1) / kBlockK;
-    int64_t nkb;
-    if (g.tile) {
-        p.tn = fp4 ? 192 : 256;
-        p.units = static_cast<int32_t>((n + kTileRows - 1) / kTileRows);
-        p.piece_units = 1;
-        p.w_stage = kTileRows * kBlockK;
-        p.x_stage = p.tn * kBlockK;
-        nkb = k_chunks;
+    const int chunks = g.pair ? 1 : 4;  // of a stage
+    const int64_t nkb = (k_chunks + chunks - 1) / chunks;
+    // Bytes in front of the W ring that an MMA may read: a piece that starts
+    // inside a scale block stands that many rows into the MMA's rows.
+    const uint32_t front = fp4 && !g.pair ? kTileRows * kBlockK : 0;
+    if (g.pair) {
+        p.tn = 256;
+        p.units = static_cast<int32_t>((n + 2 * kTileRows - 1) / (2 * kTileRows));
+        p.piece_units = kBlockUnits;
+        p.x_stage = p.tn / 2 * kBlockK;
+        // Two accumulators.  With the scales' 64 columns there is no room for
+        // two of 256: the second starts at column 192, and the epilogue
+        // empties the 64 columns that both use first.
+        p.acc_cols = fp4 ? 192 : 256;
+        p.sf_col = 448;
+        p.tmem_cols = 512;
     } else {
         p.tn = static_cast<int32_t>(std::min<int64_t>(64, (3 * avg + 15) / 16 * 16));
-        p.units = static_cast<int32_t>((n + 7) / 8);
-        const int64_t share = (groups * p.units + sm_count - 1) / sm_count;
-        p.piece_units = static_cast<int32_t>(std::min<int64_t>(16, share));
-        p.w_stage = p.piece_units * 8 * 4 * kBlockK;
-        p.x_stage = p.tn * 4 * kBlockK;
+        const int64_t n_units = (n + 7) / 8, blocks = (n_units + kBlockUnits - 1) / kBlockUnits;
+        p.units = static_cast<int32_t>(n_units);
+        p.blocked = fp4 ? 1 : 0;
         p.chunked = k_bytes % kBlockK == 0;
-        nkb = (k_chunks + 3) / 4;
+        if (fp4 && groups * blocks < sm_count) {
+            // Less than a block per SM: equal parts of a block, one piece each
+            // (a share that crosses a block would take two passes over K).
+            const int per = static_cast<int>(std::min<int64_t>(kBlockUnits, sm_count / (groups * blocks)));
+            p.part_units = (kBlockUnits + per - 1) / per;
+            p.units = static_cast<int32_t>(blocks * ((kBlockUnits + p.part_units - 1) / p.part_units));
+            p.piece_units = p.part_units;
+        } else {
+            const int64_t share = (groups * n_units + sm_count - 1) / sm_count;
+            p.piece_units = static_cast<int32_t>(fp4 ? kBlockUnits : std::min<int64_t>(kBlockUnits, share));
+        }
+        int x_rows = 8;
+        while (x_rows < p.tn) x_rows *= 2;
+        p.x_stage = x_rows * chunks * kBlockK;
+        p.acc_cols = static_cast<uint32_t>(p.tn);
+        p.sf_col = 2 * p.acc_cols;
+        p.tmem_cols = 32;
+        while (p.tmem_cols < 2 * p.acc_cols + (fp4 ? 2 * kSfSlotCols : 0)) p.tmem_cols *= 2;
     }
-    if (fp4)
-        p.sf_stage = (g.tile ? 1 : 4) * 2 * (1 + grouped_x_scale_blocks(g.tile)) * kScaleBlock;
-    const int64_t max_tiles = groups + rows / p.tn;
-    if (max_tiles * p.units > (int64_t(1) << 31) - (int64_t(1) << 20)) return "too many tiles";
-    g.grid = static_cast<int>(std::min<int64_t>(sm_count, max_tiles * p.units));
-    p.acc_cols = static_cast<uint32_t>(p.tn);
-    p.sf_col = 2 * p.acc_cols;
-    p.tmem_cols = 32;
-    while (p.tmem_cols < 2 * p.acc_cols + (fp4 ? 2 * kSfSlotCols : 0)) p.tmem_cols *= 2;
+    p.w_stage = p.piece_units * chunks * 1024;
+    if (fp4) p.sf_stage = chunks * 2 * (1 + grouped_x_scale_blocks(g.pair)) * kScaleBlock;
+    const int64_t max_items = (groups + rows / p.tn) * p.units;
+    if (max_items > (int64_t(1) << 31) - (int64_t(1) << 20)) return "too many tiles";
+    g.grid = static_cast<int>(g.pair ? 2 * std::min<int64_t>(sm_count / 2, max_items)
+                                     : std::min<int64_t>(sm_count, max_items));
 
     const uint32_t tables = 8u * static_cast<uint32_t>(experts + 1);
     auto bytes_for = [&](int stages) -> uint32_t {
         p.stages = stages;
-        p.sf_off = static_cast<uint32_t>(stages * (p.w_stage + p.x_stage));
-        p.bar_off = p.sf_off + static_cast<uint32_t>(stages * p.sf_stage);
-        p.tab_off = p.bar_off + 8u * (3 * stages + 5) + 8u;
-        // The MMA reads 128 W rows whatever the piece holds: the last stage's
-        // read has to end inside the allocation.
-        const uint32_t read_end = static_cast<uint32_t>((stages - 1) * p.w_stage) +
-                                  kTileRows * kBlockK * (g.tile ? 1u : 4u);
-        return std::max(p.tab_off + tables, read_end) + 1024u;
+        p.sf_off = static_cast<uint32_t>(stages * p.x_stage);
+        p.w_off = p.sf_off + static_cast<uint32_t>(stages * p.sf_stage);
+        p.w_off = (std::max(p.w_off, front) + 1023u) & ~1023u;
+        p.bar_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
+        p.tab_off = p.bar_off + 8u * (2 * stages + kGrpBars) + 8u;
+        // The MMA's 128 W rows of the last chunk end inside the allocation.
+        const uint32_t read_end = p.w_off + static_cast<uint32_t>(stages * p.w_stage) + kTileRows * kBlockK;
+        return std::max(p.tab_off + tables, g.pair ? 0u : read_end) + 1024u;
     };
     int stages = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(12, 2 * nkb)));
     while (stages >= 2 && bytes_for(stages) > smem_limit) --stages;
@@ -219,24 +284,65 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     return nullptr;
 }
 
-// K-major SW128 operand whose 8-row groups lie `sbo` bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t smem_addr, uint32_t sbo) {
-    return (sw128_kmajor_desc(smem_addr) & ~(0x3FFFull << 32)) |
-           (static_cast<uint64_t>(sbo >> 4) << 32);
-}
-
 // Unswizzled 32 rows x 16 bytes (a scale block): 8-row groups 128 bytes apart.
 __device__ __forceinline__ uint64_t scale_desc(uint32_t smem_addr) {
     return static_cast<uint64_t>((smem_addr >> 4) & 0x3FFFu) |
            (static_cast<uint64_t>(128u >> 4) << 32) | (static_cast<uint64_t>(1u) << 46);
 }
 
-// One 512-byte scale block to 4 TMEM columns, repeated in the four 32-lane
-// subpartitions: lane i, column j gets the four scales of row 32 j + i.
-__device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
-    asm volatile("tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;" ::"r"(taddr), "l"(desc)
-                 : "memory");
-}
+// tcgen05 operations of one CTA, or of both CTAs of a pair.
+template <int CTAS>
+struct Tc;
+#define TINYM_TC_OPS(G)                                                                            \
+    template <>                                                                                    \
+    struct Tc<G> {                                                                                 \
+        /* 512-byte scale block to 4 TMEM columns, repeated in the four 32-lane subpartitions: */  \
+        /* lane i, column j gets the four scales of row 32 j + i. */                               \
+        __device__ __forceinline__ static void cp_scales(uint32_t taddr, uint64_t desc) {          \
+            asm volatile("tcgen05.cp.cta_group::" #G ".32x128b.warpx4 [%0], %1;" ::"r"(taddr),     \
+                         "l"(desc)                                                                 \
+                         : "memory");                                                              \
+        }                                                                                          \
+        __device__ __forceinline__ static void mma_e4m3(uint32_t d, uint64_t a, uint64_t b,        \
+                                                        uint32_t idesc, uint32_t accumulate) {     \
+            asm volatile(                                                                          \
+                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"                                 \
+                "tcgen05.mma.cta_group::" #G ".kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d), \
+                "l"(a), "l"(b), "r"(idesc), "r"(accumulate)                                        \
+                : "memory");                                                                       \
+        }                                                                                          \
+        __device__ __forceinline__ static void mma_mxf4(uint32_t d, uint64_t a, uint64_t b,        \
+                                                        uint32_t idesc, uint32_t sfa, uint32_t sfb, \
+                                                        uint32_t accumulate) {                     \
+            asm volatile(                                                                          \
+                "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %6, 0;\n\t"                                 \
+                "tcgen05.mma.cta_group::" #G                                                       \
+                ".kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], [%5], p;\n\t}\n" ::  \
+                    "r"(d),                                                                        \
+                "l"(a), "l"(b), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)                    \
+                : "memory");                                                                       \
+        }                                                                                          \
+        __device__ __forceinline__ static void commit(uint32_t bar) {                              \
+            asm volatile("tcgen05.commit.cta_group::" #G                                           \
+                         ".mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar)             \
+                         : "memory");                                                              \
+        }                                                                                          \
+        __device__ __forceinline__ static void alloc(uint32_t dst, uint32_t ncols) {               \
+            asm volatile("tcgen05.alloc.cta_group::" #G                                            \
+                         ".sync.aligned.shared::cta.b32 [%0], %1;\n\t"                             \
+                         "tcgen05.relinquish_alloc_permit.cta_group::" #G ".sync.aligned;" ::"r"(dst), \
+                         "r"(ncols)                                                                \
+                         : "memory");                                                              \
+        }                                                                                          \
+        __device__ __forceinline__ static void dealloc(uint32_t taddr, uint32_t ncols) {           \
+            asm volatile("tcgen05.dealloc.cta_group::" #G ".sync.aligned.b32 %0, %1;" ::"r"(taddr), \
+                         "r"(ncols)                                                                \
+                         : "memory");                                                              \
+        }                                                                                          \
+    };
+TINYM_TC_OPS(1)
+TINYM_TC_OPS(2)
+#undef TINYM_TC_OPS
 
 // Instruction descriptor of kind::mxf4: A = B = E2M1 (1) at [7,10) and
 // [10,13), N >> 3 at [17,23), E8M0 scales (1) at 23, M >> 7 at [27,29).
@@ -245,17 +351,6 @@ __device__ __forceinline__ void tmem_cp_scales(uint32_t taddr, uint64_t desc) {
 __host__ __device__ constexpr uint32_t idesc_mxf4(int mma_m, int mma_n) {
     return (1u << 7) | (1u << 10) | (static_cast<uint32_t>(mma_n >> 3) << 17) | (1u << 23) |
            (static_cast<uint32_t>(mma_m >> 7) << 27);
-}
-__device__ __forceinline__ void umma_mxf4(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
-                                          uint32_t idesc, uint32_t sfa, uint32_t sfb,
-                                          uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %6, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X [%0], %1, %2, %3, [%4], "
-        "[%5], p;\n\t}\n" ::"r"(d_tmem),
-        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(sfa), "r"(sfb), "r"(accumulate)
-        : "memory");
 }
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
@@ -269,8 +364,60 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
+// Arrive on a barrier of another CTA of the cluster (a cluster address), with
+// the default release at CTA scope: what it announces (bulk copies that have
+// landed in this CTA's shared memory, scales behind a proxy fence, tensor
+// memory that has been read) is complete in this SM when it is sent, and only
+// tensor-core operations that the other CTA issues later depend on it.  A
+// release at cluster scope took ~1,000 cycles here, twice a stage's MMAs.
+__device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// Bounded wait of a whole warp: no lane diverges and the outcome is uniform.
+// CLUSTER: other CTAs of the cluster arrive on the barrier.  The clock that
+// bounds it is first read after many tries: a read of %globaltimer costs
+// several hundred cycles even where its value is not used.
+template <bool CLUSTER>
+__device__ __forceinline__ bool warp_try(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    if constexpr (CLUSTER) {
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}\n"
+            : "=r"(ok)
+            : "r"(bar), "r"(parity)
+            : "memory");
+    } else {
+        ok = mbar_try_wait(bar, parity) ? 1u : 0u;
+    }
+    return __all_sync(0xFFFFFFFFu, ok);
+}
+// Called now and then while a wait lasts; false: give up.
+__device__ __noinline__ bool warp_wait_tick(uint64_t* t0, const WaitGuard& g, uint32_t code) {
+    if (__any_sync(0xFFFFFFFFu, *g.abort)) return false;
+    const uint64_t t = __shfl_sync(0xFFFFFFFFu, globaltimer_ns(), 0);
+    if (*t0 == 0) *t0 = t;
+    if (t - *t0 <= g.timeout_ns) return true;
+    *g.abort = 1u;
+    if ((threadIdx.x & 31) == 0) report_timeout(g.err_word, g.err_host, code);
+    return false;
+}
+template <bool CLUSTER = false>
+__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const WaitGuard& g,
+                                          uint32_t code) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 1; !warp_try<CLUSTER>(bar, parity); ++it)
+        if ((it & 255u) == 0 && !warp_wait_tick(&t0, g, code)) return false;
+    return true;
+}
+
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() {
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -280,7 +427,7 @@ __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-__device__ __forceinline__ void tmem_ld_x16_nowait(uint32_t taddr, uint32_t (&r)[16]) {
+__device__ __forceinline__ void tmem_ld_x16_nowait(uint32_t taddr, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
         "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
@@ -335,66 +482,62 @@ __device__ __forceinline__ void grouped_tables(const GroupedParams& p, int32_t* 
     }
 }
 
-template <bool FP4, bool TILE>
+template <bool FP4, bool PAIR>
 __global__ void __launch_bounds__(kGrpThreads, 1)
-    tinym_grouped_kernel(const __grid_constant__ CUtensorMap tm_w,
-                         const __grid_constant__ CUtensorMap tm_x, const GroupedParams p) {
-    // Bytes of K per stage in 128-byte chunks; rows of one W and one X box.
-    constexpr int kChunks = TILE ? 1 : 4;
-    constexpr int kXBox = TILE ? 32 : 8;
-    // Operand layout of a stage: 8-row swizzle atoms of 1024 bytes; the four
-    // chunks of a unit are consecutive in a stream stage.
-    constexpr uint32_t kSbo = kChunks * 1024;
-    constexpr int kMmaK = 32;        // bytes of K per MMA (32 E4M3 or 64 E2M1 elements)
-    constexpr int kSfPerChunk = 2;   // MXFP4: scale blocks (128 elements) per chunk
-    constexpr int kXsBlocks = grouped_x_scale_blocks(TILE);
+    tinym_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) {
+    using Ops = Tc<PAIR ? 2 : 1>;
+    constexpr int kCtas = PAIR ? 2 : 1;
+    constexpr int kChunks = PAIR ? 1 : 4;  // 128-byte chunks of K per stage
+    constexpr int kMmaK = 32;              // bytes of K per MMA (32 E4M3 or 64 E2M1 elements)
+    constexpr int kSfPerChunk = 2;         // MXFP4: scale blocks (128 elements) per chunk
+    constexpr int kXsBlocks = grouped_x_scale_blocks(PAIR);
+    constexpr int kWsBytes = kChunks * kSfPerChunk * kScaleBlock;  // W scales of a stage
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = align1024(smem_raw);
     const uint32_t s_base = smem_u32(smem);
     const int stages = p.stages;
-    const uint32_t w_ring = s_base;
-    const uint32_t x_ring = s_base + stages * p.w_stage;
+    const uint32_t x_ring = s_base;
     const uint32_t sf_ring = s_base + p.sf_off;
+    const uint32_t w_ring = s_base + p.w_off;
     const uint32_t bars = s_base + p.bar_off;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
-    auto sf_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
-    auto acc_full = [&](int b) { return bars + 8u * (3 * stages + b); };
-    auto acc_empty = [&](int b) { return bars + 8u * (3 * stages + 2 + b); };
-    const uint32_t drain_bar = bars + 8u * (3 * stages + 4);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (3 * stages + 5));
+    auto acc_full = [&](int b) { return bars + 8u * (2 * stages + b); };
+    auto acc_empty = [&](int b) { return bars + 8u * (2 * stages + 2 + b); };
+    auto acc_part = [&](int b) { return bars + 8u * (2 * stages + 4 + b); };
+    const uint32_t drain_bar = bars + 8u * (2 * stages + 6);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (2 * stages + kGrpBars));
     volatile uint32_t* abort_flag = tmem_slot + 1;
     int32_t* off = reinterpret_cast<int32_t*>(smem + p.tab_off);
     int32_t* prefix = off + p.experts + 1;
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
+    const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;  // 0 issues the pair's MMAs
     const WaitGuard guard{abort_flag, &g_err_word, p.timeout_ns, p.err_host};
     const int k_chunks = (p.k_bytes + kBlockK - 1) / kBlockK;
     const int nkb = (k_chunks + kChunks - 1) / kChunks;
+    auto at_rank = [&](uint32_t addr, int r) { return PAIR ? dsmem_map(addr, r) : addr; };
 
     if (threadIdx.x == 0) {
-        tma_prefetch_desc(&tm_w);
-        tma_prefetch_desc(&tm_x);
         for (int s = 0; s < stages; ++s) {
-            mbar_init(full_bar(s), 1);
+            // full: the producer's expect_tx (and the bytes), the two scale
+            // warps, and at CTA 0 of a pair the stage of CTA 1
+            mbar_init(full_bar(s), 1 + (FP4 ? 2 : 0) + (PAIR && rank == 0 ? 1 : 0));
             mbar_init(empty_bar(s), 1);
-            mbar_init(sf_bar(s), 2);  // one arrival per scale warp
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
-            mbar_init(acc_empty(b), 4);  // one arrival per epilogue warp
+            mbar_init(acc_empty(b), 4 * kCtas);  // one arrival per epilogue warp
+            mbar_init(acc_part(b), 4 * kCtas);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0u;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
-    if (warp == 1) {
-        tmem_alloc(smem_u32(tmem_slot), p.tmem_cols);
-        tmem_relinquish();
-    }
+    if (warp == 1) Ops::alloc(smem_u32(tmem_slot), p.tmem_cols);
     // Everything above overlaps the previous kernel's tail (programmatic
     // dependent launch); no global memory is read before it has completed.
     grid_dependency_wait();
@@ -402,222 +545,272 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     if (warp == 2) grouped_tables(p, off, prefix, lane);
     tc_fence_before_sync();
     __syncthreads();
+    if constexpr (PAIR) {  // the other CTA's barriers exist before anything arrives on them
+        cluster_arrive_release();
+        cluster_wait_acquire();
+    }
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    GroupedWalk<TILE> walk(p, off, prefix, blockIdx.x, gridDim.x);
+    GroupedWalk<PAIR> walk(p, off, prefix, blockIdx.x / kCtas, gridDim.x / kCtas);
     GroupedPiece w;
+    // MMA row of a stream piece's first W row (0 unless scales are blocked).
+    auto first_row = [&]() { return !PAIR && FP4 ? w.w0 % kTileRows : 0; };
+    // X rows that this CTA loads, and the box that holds them.
+    auto x_cols = [&]() { return PAIR ? ((w.rows + 31) & ~31) / 2 : w.rows; };
+    auto x_box = [&](int cols) {
+        int i = 0;
+        while (grouped_x_box(PAIR, i) < cols) ++i;
+        return i;
+    };
+
     if (warp == 0) {
-        // ---------------- TMA producer
-        if (lane == 0) {
-            const uint64_t pol_w = TILE ? l2_policy_evict_normal() : l2_policy_w();
-            const uint64_t pol_x = l2_policy_evict_last();
-            int s = 0, issued = 0;
-            uint32_t ph = 1u;  // the first pass over the ring does not wait
-            bool ok = true;
-            while (ok && walk.next(&w)) {
-                const int w_units = TILE ? 1 : w.h / 8;
-                const int x_boxes = (w.rows + kXBox - 1) / kXBox;
-                for (int i = 0; i < nkb; ++i) {
-                    if (!(ok = mbar_wait_inline(empty_bar(s), ph, guard, kErrProducerWait, true)))
-                        break;
-                    const uint32_t wd = w_ring + s * p.w_stage, xd = x_ring + s * p.x_stage;
-                    const uint32_t bar = full_bar(s);
-                    const int c0 = i * kChunks;
-                    if constexpr (TILE) {
-                        mbar_expect_tx(bar, kTileRows * kBlockK + x_boxes * kXBox * kBlockK);
-                        tma_load_3d(wd, &tm_w, bar, c0 * kBlockK, w.w0, w.e, pol_w);
-                        for (int b = 0; b < x_boxes; ++b)
-                            tma_load_3d(xd + b * kXBox * kBlockK, &tm_x, bar, c0 * kBlockK,
-                                        w.row0 + b * kXBox, 0, pol_x);
+        // ---------------- TMA producer (the whole warp walks, one lane issues)
+        const uint64_t pol_w = PAIR ? l2_policy_evict_normal() : l2_policy_w();
+        const uint64_t pol_x = l2_policy_evict_last();
+        int s = 0, issued = 0;
+        uint32_t ph = 1u;  // the first pass over the ring does not wait
+        bool ok = true;
+        while (ok && walk.next(&w)) {
+            const int cols = x_cols();
+            const int xi = x_box(cols);
+            const int x_rows = grouped_x_box(PAIR, xi);
+            const int x_row = w.row0 + rank * cols;
+            const int w_rows = PAIR ? kTileRows : w.h;
+            const int w_row = w.w0 + rank * kTileRows;
+            const CUtensorMap* mw = &maps.w[w_rows / 8 - 1];
+            const CUtensorMap* mx = &maps.x[xi];
+            for (int i = 0; i < nkb; ++i) {
+                if (!(ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait))) break;
+                const uint32_t wd = w_ring + s * p.w_stage, xd = x_ring + s * p.x_stage;
+                const uint32_t bar = full_bar(s);
+                const int c0 = i * kChunks;
+                if (elect_one()) {
+                    // Only CTA 0 sees the MMAs retire: it passes the free slot on.
+                    if (PAIR && rank == 0 && issued >= stages)
+                        mbar_arrive_remote(at_rank(empty_bar(s), 1));
+                    if constexpr (PAIR) {
+                        mbar_expect_tx(bar, (kTileRows + x_rows) * kBlockK);
+                        tma_load_3d(wd, mw, bar, c0 * kBlockK, w_row, w.e, pol_w);
+                        tma_load_3d(xd, mx, bar, c0 * kBlockK, x_row, 0, pol_x);
                     } else if (p.chunked) {
-                        mbar_expect_tx(bar, (w_units + x_boxes) * kChunks * 1024);
-                        for (int b = 0; b < x_boxes; ++b)
-                            tma_load_4d(xd + b * kChunks * 1024, &tm_x, bar, 0, w.row0 + b * 8, c0,
-                                        0, pol_x);
-                        for (int b = 0; b < w_units; ++b)
-                            tma_load_4d(wd + b * kChunks * 1024, &tm_w, bar, 0, w.w0 + b * 8, c0,
-                                        w.e, pol_w);
+                        mbar_expect_tx(bar, (w_rows + x_rows) * kChunks * kBlockK);
+                        tma_load_4d(wd, mw, bar, 0, w_row, c0, w.e, pol_w);
+                        tma_load_4d(xd, mx, bar, 0, x_row, c0, 0, pol_x);
                     } else {
                         const int nc = min(kChunks, k_chunks - c0);
-                        mbar_expect_tx(bar, (w_units + x_boxes) * nc * 1024);
-                        for (int b = 0; b < x_boxes; ++b)
-                            for (int c = 0; c < nc; ++c)
-                                tma_load_3d(xd + (b * kChunks + c) * 1024, &tm_x, bar,
-                                            (c0 + c) * kBlockK, w.row0 + b * 8, 0, pol_x);
-                        for (int b = 0; b < w_units; ++b)
-                            for (int c = 0; c < nc; ++c)
-                                tma_load_3d(wd + (b * kChunks + c) * 1024, &tm_w, bar,
-                                            (c0 + c) * kBlockK, w.w0 + b * 8, w.e, pol_w);
+                        mbar_expect_tx(bar, (w_rows + x_rows) * nc * kBlockK);
+                        for (int c = 0; c < nc; ++c) {
+                            tma_load_3d(wd + c * w_rows * kBlockK, mw, bar, (c0 + c) * kBlockK, w_row,
+                                        w.e, pol_w);
+                            tma_load_3d(xd + c * x_rows * kBlockK, mx, bar, (c0 + c) * kBlockK, x_row,
+                                        0, pol_x);
+                        }
                     }
-                    ++issued;
+                }
+                __syncwarp();
+                ++issued;
+                if (++s == stages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
+        }
+        if (lane == 0 && *abort_flag) {
+            // Wait (bounded) for the copies still in flight before shared
+            // memory is released; a stage that lacks another arrival runs
+            // into the limit, long after every copy has landed.
+            for (int j = max(0, issued - stages); j < issued; ++j)
+                if (!mbar_drain(full_bar(j % stages), (j / stages) & 1, guard, kErrDrain)) break;
+        }
+    } else if (warp == 1) {
+        // ---------------- MMA issuer (the whole warp walks, one lane issues)
+        if (rank == 0) {
+            const uint32_t tmem_u = __shfl_sync(0xFFFFFFFFu, tmem, 0);
+            const uint64_t da0 = sw128_kmajor_desc(w_ring);
+            const uint64_t db0 = sw128_kmajor_desc(x_ring);
+            int s = 0, piece = 0, slot = 0, last_cols = 0;
+            uint32_t ph = 0u;
+            bool ok = true;
+            while (ok && walk.next(&w)) {
+                const int b = piece & 1;
+                const uint32_t mma_n = PAIR ? (w.rows + 31) & ~31 : (w.rows + 15) & ~15;
+                const uint32_t idesc = FP4 ? idesc_mxf4(kCtas * 128, mma_n)
+                                           : idesc_e4m3_f32(kCtas * 128, mma_n);
+                const uint32_t acc = tmem_u + b * p.acc_cols;
+                const bool two = PAIR && mma_n > 128;  // X scale blocks of the tile
+                // The piece's own accumulator is free, and so are the columns
+                // that it shares with the one before.
+                const int lower = b ? last_cols : static_cast<int>(mma_n);  // columns used of buffer 0
+                ok = warp_wait<PAIR>(acc_empty(b), ((piece >> 1) & 1) ^ 1u, guard, kErrMmaWait);
+                if (PAIR && FP4 && ok && piece > 0 && lower > static_cast<int>(p.acc_cols))
+                    ok = warp_wait<PAIR>(acc_part(b ^ 1), ((piece - 1) >> 1) & 1, guard, kErrMmaWait);
+                if (!ok) break;
+                last_cols = mma_n;
+                tc_fence_after_sync();
+                // Bytes from chunk to chunk of a stage, and of the rows that
+                // stand in front of a blocked piece's first one.
+                const int w_chunk = (PAIR ? kTileRows : w.h) * kBlockK;
+                const int x_chunk = grouped_x_box(PAIR, x_box(x_cols())) * kBlockK;
+                const uint64_t da1 = da0 - static_cast<uint64_t>((first_row() * kBlockK) >> 4);
+                for (int i = 0; i < nkb; ++i) {
+                    if (!(ok = warp_wait<PAIR>(full_bar(s), ph, guard, kErrMmaWait))) break;
+                    tc_fence_after_sync();
+                    const uint64_t da = da1 + static_cast<uint64_t>((s * p.w_stage) >> 4);
+                    const uint64_t db = db0 + static_cast<uint64_t>((s * p.x_stage) >> 4);
+                    const uint32_t sf = sf_ring + s * p.sf_stage;
+                    const int nc = min(kChunks, k_chunks - i * kChunks);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int c = 0; c < kChunks; ++c) {
+                            if (c >= nc) break;
+                            uint32_t sfa = 0, sfb = 0;
+                            if constexpr (FP4) {
+                                // this chunk's scales: 2 blocks of W, 2 or 4 of X
+                                sfa = tmem_u + p.sf_col + ((slot + c) & 1) * kSfSlotCols;
+                                sfb = sfa + 4 * kSfPerChunk;
+#pragma unroll
+                                for (int q = 0; q < kSfPerChunk; ++q) {
+                                    const int blk = c * kSfPerChunk + q;
+                                    const uint32_t xs = sf + kWsBytes + blk * kXsBlocks * kScaleBlock;
+                                    Ops::cp_scales(sfa + 4 * q, scale_desc(sf + blk * kScaleBlock));
+                                    Ops::cp_scales(sfb + 8 * q, scale_desc(xs));
+                                    if (PAIR && two)
+                                        Ops::cp_scales(sfb + 8 * q + 4, scale_desc(xs + kScaleBlock));
+                                }
+                            }
+#pragma unroll
+                            for (int kk = 0; kk < kBlockK / kMmaK; ++kk) {
+                                const uint64_t ak = da + static_cast<uint64_t>((c * w_chunk + kk * kMmaK) >> 4);
+                                const uint64_t bk = db + static_cast<uint64_t>((c * x_chunk + kk * kMmaK) >> 4);
+                                const uint32_t accumulate = (i | c | kk) ? 1u : 0u;
+                                if constexpr (FP4) {
+                                    // 64 elements: scales 2 (kk % 2), +1 of block kk / 2
+                                    const uint32_t id = (kk & 1) * 2;
+                                    Ops::mma_mxf4(acc, ak, bk, idesc | (id << 4) | (id << 29),
+                                                  sfa + 4 * (kk >> 1), sfb + 8 * (kk >> 1), accumulate);
+                                } else {
+                                    Ops::mma_e4m3(acc, ak, bk, idesc, accumulate);
+                                }
+                            }
+                        }
+                        Ops::commit(empty_bar(s));
+                        if (i == nkb - 1) Ops::commit(acc_full(b));
+                    }
+                    __syncwarp();
+                    slot += kChunks;
+                    if (++s == stages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+                ++piece;
+            }
+            if (!ok) {
+                // An abort: wait for every MMA issued so far.
+                if (elect_one()) Ops::commit(drain_bar);
+                __syncwarp();
+                if (lane == 0) mbar_drain(drain_bar, 0, guard, kErrDrain);
+                __syncwarp();
+            }
+        } else {
+            // CTA 1: pass the arrival of its data and scales on to CTA 0.
+            int s = 0;
+            uint32_t ph = 0u;
+            bool ok = true;
+            while (ok && walk.next(&w)) {
+                for (int i = 0; i < nkb; ++i) {
+                    if (!(ok = warp_wait(full_bar(s), ph, guard, kErrMmaWait))) break;
+                    if (elect_one()) mbar_arrive_remote(at_rank(full_bar(s), 0));
+                    __syncwarp();
                     if (++s == stages) {
                         s = 0;
                         ph ^= 1u;
                     }
                 }
             }
-            if (*abort_flag) {
-                // Drain the copies still in flight before shared memory is released.
-                for (int j = max(0, issued - stages); j < issued; ++j)
-                    mbar_drain(full_bar(j % stages), (j / stages) & 1, guard, kErrDrain);
-            }
-        }
-    } else if (warp == 1) {
-        // ---------------- MMA issuer (the whole warp walks, one lane issues)
-        const uint32_t tmem_u = __shfl_sync(0xFFFFFFFFu, tmem, 0);
-        const uint64_t da0 = sw128_desc(w_ring, kSbo);
-        const uint64_t db0 = sw128_desc(x_ring, kSbo);
-        int s = 0, piece = 0, slot = 0;
-        uint32_t ph = 0u;
-        bool ok = true;
-        while (ok && walk.next(&w)) {
-            const int b = piece & 1;
-            const uint32_t mma_n = (w.rows + 15) & ~15;
-            const uint32_t idesc = FP4 ? idesc_mxf4(128, mma_n) : idesc_e4m3_f32(128, mma_n);
-            const uint32_t acc = tmem_u + b * p.acc_cols;
-            const bool two = mma_n > 128;  // X scale blocks of the tile
-            if (lane == 0)
-                ok = mbar_wait_inline(acc_empty(b), ((piece >> 1) & 1) ^ 1u, guard, kErrMmaWait, true);
-            if (!(ok = __shfl_sync(0xFFFFFFFFu, ok, 0))) break;
-            tc_fence_after_sync();
-            for (int i = 0; i < nkb; ++i) {
-                if (lane == 0) {
-                    ok = mbar_wait_inline(full_bar(s), ph, guard, kErrMmaWait, true);
-                    if (FP4 && ok)
-                        ok = mbar_wait_inline(sf_bar(s), ph, guard, kErrMmaWait, true);
-                }
-                if (!(ok = __shfl_sync(0xFFFFFFFFu, ok, 0))) break;
-                tc_fence_after_sync();
-                const uint64_t da = da0 + static_cast<uint64_t>((s * p.w_stage) >> 4);
-                const uint64_t db = db0 + static_cast<uint64_t>((s * p.x_stage) >> 4);
-                const uint32_t sf = sf_ring + s * p.sf_stage;
-                const int nc = min(kChunks, k_chunks - i * kChunks);
-                if (elect_one()) {
-#pragma unroll
-                    for (int c = 0; c < kChunks; ++c) {
-                        if (c >= nc) break;
-                        uint32_t sfa = 0, sfb = 0;
-                        if constexpr (FP4) {
-                            // this chunk's scales: 2 blocks of W, 2 or 4 of X
-                            sfa = tmem_u + p.sf_col + ((slot + c) & 1) * kSfSlotCols;
-                            sfb = sfa + 4 * kSfPerChunk;
-                            const uint32_t xs = sf + kChunks * kSfPerChunk * kScaleBlock;
-#pragma unroll
-                            for (int q = 0; q < kSfPerChunk; ++q) {
-                                tmem_cp_scales(sfa + 4 * q,
-                                               scale_desc(sf + (c * kSfPerChunk + q) * kScaleBlock));
-                                tmem_cp_scales(sfb + 8 * q,
-                                               scale_desc(xs + (c * kSfPerChunk + q) * kXsBlocks * kScaleBlock));
-                                if (TILE && two)
-                                    tmem_cp_scales(
-                                        sfb + 8 * q + 4,
-                                        scale_desc(xs + ((c * kSfPerChunk + q) * kXsBlocks + 1) * kScaleBlock));
-                            }
-                        }
-#pragma unroll
-                        for (int kk = 0; kk < kBlockK / kMmaK; ++kk) {
-                            const uint64_t step = static_cast<uint64_t>((c * 1024 + kk * kMmaK) >> 4);
-                            const uint32_t accumulate = (i | c | kk) ? 1u : 0u;
-                            if constexpr (FP4) {
-                                // 64 elements: scales 2 (kk % 2), +1 of block kk / 2
-                                const uint32_t id = (kk & 1) * 2;
-                                umma_mxf4(acc, da + step, db + step, idesc | (id << 4) | (id << 29),
-                                          sfa + 4 * (kk >> 1), sfb + 8 * (kk >> 1), accumulate);
-                            } else {
-                                umma_e4m3(acc, da + step, db + step, idesc, accumulate);
-                            }
-                        }
-                    }
-                    umma_commit(empty_bar(s));
-                    if (i == nkb - 1) umma_commit(acc_full(b));
-                }
-                __syncwarp();
-                slot += kChunks;
-                if (++s == stages) {
-                    s = 0;
-                    ph ^= 1u;
-                }
-            }
-            ++piece;
-        }
-        if (!ok) {
-            // An abort: wait for every MMA issued so far.
-            if (elect_one()) umma_commit(drain_bar);
-            __syncwarp();
-            if (lane == 0) mbar_drain(drain_bar, 0, guard, kErrDrain);
-            __syncwarp();
         }
     } else if (warp < 4) {
-        // ---------------- MXFP4 scales: 4-byte words (128 elements of a row)
-        // gathered into the 128-row block order that tcgen05.cp takes, since a
-        // piece may start at any row.  Warp 2 and 3 take alternate blocks of K.
+        // ---------------- MXFP4 scales.  Warps 2 and 3 take alternate blocks of
+        // K: a block of W as it lies in memory (one 16-byte copy per lane), X
+        // rows as 4-byte words gathered into the block order.
         if constexpr (FP4) {
             const int blocks = (p.k_bytes * 2 + 127) / 128;     // scale blocks along K
             const int tail = (p.k_bytes * 2 % 128) / 32;        // scales in the last one, 0: all
+            const uint32_t tail_mask = tail ? (1u << (8 * tail)) - 1u : 0xFFFFFFFFu;
             int s = 0, pending = 0, ps = 0;
             uint32_t ph = 1u;
             bool ok = true;
-            auto arrive = [&](int slot_) {
+            auto arrive = [&]() {  // the oldest pending stage
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(sf_bar(slot_));
+                if (lane == 0) mbar_arrive(full_bar(ps));
+                if (++ps == stages) ps = 0;
+                --pending;
             };
             auto flush = [&]() {
                 cp_async_wait<0>();
-                for (; pending > 0; --pending) {
-                    arrive(ps);
-                    if (++ps == stages) ps = 0;
-                }
+                while (pending > 0) arrive();
             };
             while (ok && walk.next(&w)) {
-                const uint8_t* ws = p.w_scales + w.e * p.w_scale_stride;
-                const int w_groups = (min(w.h, p.n - w.w0) + 31) / 32;
+                const int w0 = w.w0 + rank * kTileRows;
+                const uint8_t* ws = p.w_scales + w.e * p.w_scale_stride +
+                                    static_cast<int64_t>(w0 >> 7) * blocks * kScaleBlock + lane * 16;
+                const bool w_in = w0 < p.n;
                 const int x_groups = (w.rows + 31) / 32;
                 for (int i = 0; i < nkb; ++i) {
-                    if (!__all_sync(0xFFFFFFFFu, mbar_try_wait(empty_bar(s), ph))) {
+                    if (!warp_try<PAIR>(empty_bar(s), ph)) {
                         flush();  // before blocking: the MMA may need what is pending
-                        ok = __all_sync(0xFFFFFFFFu, mbar_wait(empty_bar(s), ph, guard, kErrProducerWait));
+                        ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait);
                         if (!ok) break;
                     }
                     const uint32_t sf = sf_ring + s * p.sf_stage;
-                    const uint32_t xs = sf + kChunks * kSfPerChunk * kScaleBlock;
                     const int b0 = i * kChunks * kSfPerChunk;
-                    const int nb = min(kChunks * kSfPerChunk, blocks - b0);
-                    for (int q = warp - 2; q < kChunks * kSfPerChunk; q += 2) {
-                        const bool in = q < nb;
-                        const bool cut = in && tail && b0 + q == blocks - 1;
-                        auto word = [&](uint32_t dst, const uint8_t* base, int row) {
-                            const uint8_t* src = base +
-                                (static_cast<int64_t>(row >> 7) * blocks + b0 + q) * kScaleBlock +
-                                (row & 31) * 16 + ((row >> 5) & 3) * 4;
-                            if (in && !cut) {
-                                cp_async_4(dst, src);
-                            } else {
-                                // past K: the data are zeros, the scales 2^-127
-                                uint32_t v = in ? __ldg(reinterpret_cast<const uint32_t*>(src)) : 0u;
-                                v &= (1u << (8 * tail)) - 1u;
-                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(dst), "r"(v) : "memory");
+#pragma unroll
+                    for (int j = 0; j < kChunks * kSfPerChunk / 2; ++j) {
+                        const int q = 2 * j + warp - 2;
+                        const int kb = b0 + q;
+                        const uint32_t wd = sf + q * kScaleBlock + lane * 16;
+                        const uint32_t xd = sf + kWsBytes + q * kXsBlocks * kScaleBlock + lane * 16;
+                        if (kb < blocks - 1 || (kb == blocks - 1 && !tail)) {
+                            if (w_in) cp_async_16(wd, ws + static_cast<int64_t>(kb) * kScaleBlock);
+                            for (int g = 0; g < x_groups; ++g) {
+                                const int r = w.row0 + min(g * 32 + lane, w.rows - 1);
+                                cp_async_4(xd + (g >> 2) * kScaleBlock + (g & 3) * 4,
+                                           p.x_scales +
+                                               (static_cast<int64_t>(r >> 7) * blocks + kb) * kScaleBlock +
+                                               (r & 31) * 16 + ((r >> 5) & 3) * 4);
                             }
-                        };
-                        for (int g = 0; g < w_groups; ++g) {
-                            const int r = w.w0 + g * 32 + lane;
-                            if (r < p.n)
-                                word(sf + q * kScaleBlock + lane * 16 + g * 4, ws, r);
-                        }
-                        for (int g = 0; g < x_groups; ++g) {
-                            const int r = g * 32 + lane;
-                            if (r < w.rows)
-                                word(xs + (q * kXsBlocks + (g >> 2)) * kScaleBlock + lane * 16 + (g & 3) * 4,
-                                     p.x_scales, w.row0 + r);
+                        } else {
+                            // The last, partial block: scales past K become 2^-127
+                            // (the data there are zeros); a block past K likewise.
+                            const uint32_t mask = kb < blocks ? tail_mask : 0u;
+                            const int kc = min(kb, blocks - 1);
+                            if (w_in) {
+                                const uint4 v = __ldg(reinterpret_cast<const uint4*>(
+                                    ws + static_cast<int64_t>(kc) * kScaleBlock));
+                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(wd),
+                                             "r"(v.x & mask), "r"(v.y & mask), "r"(v.z & mask),
+                                             "r"(v.w & mask)
+                                             : "memory");
+                            }
+                            for (int g = 0; g < x_groups; ++g) {
+                                const int r = w.row0 + min(g * 32 + lane, w.rows - 1);
+                                const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(
+                                    p.x_scales +
+                                    (static_cast<int64_t>(r >> 7) * blocks + kc) * kScaleBlock +
+                                    (r & 31) * 16 + ((r >> 5) & 3) * 4));
+                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(
+                                                 xd + (g >> 2) * kScaleBlock + (g & 3) * 4),
+                                             "r"(v & mask)
+                                             : "memory");
+                            }
                         }
                     }
                     cp_async_commit();
-                    if (++pending == 3) {
-                        cp_async_wait<2>();
-                        arrive(ps);
-                        if (++ps == stages) ps = 0;
-                        --pending;
+                    if (++pending == kSfDepth) {
+                        cp_async_wait<kSfDepth - 1>();
+                        arrive();
                     }
                     if (++s == stages) {
                         s = 0;
@@ -631,33 +824,53 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         // ---------------- epilogue: warp w reads TMEM lanes 32 (w % 4) ..
         const int q = warp & 3;
         int piece = 0;
+        constexpr int kCols = PAIR ? 32 : 16;
         while (walk.next(&w)) {
             const int b = piece & 1;
-            const bool ready =
-                mbar_wait_inline(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait, true) &&
-                !*abort_flag;
-            if (!__all_sync(0xFFFFFFFFu, ready)) break;
+            if (!warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait)) break;
+            // The MMAs' commit reaches CTA 0 alone: pass it on.
+            if (PAIR && rank == 0 && warp == 4 && lane == 0)
+                mbar_arrive_remote(at_rank(acc_full(b), 1));
             tc_fence_after_sync();
             const float alpha = p.alpha ? __ldg(p.alpha + w.e * p.alpha_stride) : 1.0f;
-            const int r = q * 32 + lane;
-            const int n = w.w0 + r;
-            const bool mine = r < w.h && n < p.n;
+            const int r = q * 32 + lane - first_row();  // W row of the piece
+            const int n = w.w0 + rank * kTileRows + r;
+            const bool mine = r >= 0 && r < (PAIR ? kTileRows : w.h) && n < p.n;
             __nv_bfloat16* dst = p.y + static_cast<int64_t>(w.row0) * p.ldy + n;
             const uint32_t taddr = tmem + b * p.acc_cols + (static_cast<uint32_t>(q * 32) << 16);
-            for (int c = 0; c < w.rows; c += 16) {
-                uint32_t v[16];
-                tmem_ld_x16_nowait(taddr + c, v);
+            // Columns that both accumulators use come first: the upper ones of
+            // buffer 0, the lower ones of buffer 1.
+            const int cols = (w.rows + kCols - 1) / kCols;
+            const int shared_cols = static_cast<int>(256 - p.acc_cols) / kCols;
+            const int start = PAIR && FP4 && b == 0 && cols * kCols > static_cast<int>(p.acc_cols)
+                                  ? static_cast<int>(p.acc_cols) / kCols : 0;
+            for (int j = 0; j < cols; ++j) {
+                const int c = (j + start < cols ? j + start : j + start - cols) * kCols;
+                uint32_t v[kCols];
+#pragma unroll
+                for (int h = 0; h < kCols; h += 16) tmem_ld_x16_nowait(taddr + c + h, v + h);
                 tmem_ld_wait();
+                if (PAIR && FP4 && j == min(shared_cols, cols) - 1) {
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (rank) mbar_arrive_remote(at_rank(acc_part(b), 0));
+                        else mbar_arrive(acc_part(b));
+                    }
+                }
                 if (mine) {
 #pragma unroll
-                    for (int j = 0; j < 16; ++j)
-                        if (c + j < w.rows)
-                            dst[(c + j) * p.ldy] = __float2bfloat16_rn(__uint_as_float(v[j]) * alpha);
+                    for (int h = 0; h < kCols; ++h)
+                        if (c + h < w.rows)
+                            dst[(c + h) * p.ldy] = __float2bfloat16_rn(__uint_as_float(v[h]) * alpha);
                 }
             }
             tc_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(acc_empty(b));
+            if (lane == 0) {
+                if (PAIR && rank) mbar_arrive_remote(at_rank(acc_empty(b), 0));
+                else mbar_arrive(acc_empty(b));
+            }
             ++piece;
         }
         if (p.flags & kGrpZeroRest) {
@@ -672,9 +885,16 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     }
     __syncwarp();
     tc_fence_before_sync();
-    __syncthreads();
+    if constexpr (PAIR) {
+        // Neither CTA leaves while the other may still read its shared memory
+        // or arrive on its barriers.
+        cluster_arrive_release();
+        cluster_wait_acquire();
+    } else {
+        __syncthreads();
+    }
     tc_fence_after_sync();
-    if (warp == 1) tmem_dealloc(tmem, p.tmem_cols);
+    if (warp == 1) Ops::dealloc(tmem, p.tmem_cols);
 }
 
 }  // namespace tinym

@@ -84,6 +84,25 @@ int check_grouped(const void* x, const void* w, const void* y, int64_t ldy, int6
 }
 
 std::atomic<uint32_t> g_grouped_attr[kMaxDevices];
+std::atomic<int> g_grouped_pairs[kMaxDevices];  // CTA pairs that are resident at once (0: not asked yet)
+
+// Grid and attributes of a grouped launch; attrs holds 2 entries.
+void grouped_config(const tinym::GroupedPlan& g, void* stream, cudaLaunchConfig_t* cfg,
+                    cudaLaunchAttribute* attrs) {
+    *cfg = cudaLaunchConfig_t{};
+    cfg->gridDim = dim3(static_cast<unsigned>(g.grid));
+    cfg->blockDim = dim3(tinym::kGrpThreads);
+    cfg->dynamicSmemBytes = g.smem;
+    cfg->stream = static_cast<cudaStream_t>(stream);
+    attrs[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attrs[0].val.programmaticStreamSerializationAllowed = kUsePdl ? 1 : 0;
+    attrs[1].id = cudaLaunchAttributeClusterDimension;
+    attrs[1].val.clusterDim.x = 2;
+    attrs[1].val.clusterDim.y = 1;
+    attrs[1].val.clusterDim.z = 1;
+    cfg->attrs = attrs;
+    cfg->numAttrs = g.pair ? 2 : 1;
+}
 
 // k_bytes: bytes of one operand row.  x_scales / w_scales: MXFP4, else null.
 int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, const void* w_scales,
@@ -101,11 +120,18 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
         return fail(TINYM_ERR_UNSUPPORTED_SHAPE, "%s (rows %lld, experts %lld, N %lld)", why,
                     (long long)rows, (long long)experts, (long long)n);
     GroupedParams& p = g.prm;
-    const int chunks = !g.tile && p.chunked ? 4 : 1;
-    CUtensorMap tm_w, tm_x;
-    if ((st = encode_stack(w, experts, n, k_bytes, g.tile ? kTileRows : 8, chunks, &tm_w)) != TINYM_OK)
-        return st;
-    if ((st = encode_stack(x, 1, rows, k_bytes, g.tile ? 32 : 8, chunks, &tm_x)) != TINYM_OK) return st;
+    // A map per box height that the pieces can have.
+    const int chunks = !g.pair && p.chunked ? 4 : 1;
+    tinym::GroupedMaps maps;
+    for (int i = g.pair ? tinym::kBlockUnits - 1 : 0; i < p.piece_units; ++i)
+        if ((st = encode_stack(w, experts, n, k_bytes, 8 * (i + 1), chunks, &maps.w[i])) != TINYM_OK)
+            return st;
+    for (int i = 0; i < 4; ++i) {
+        if ((st = encode_stack(x, 1, rows, k_bytes, tinym::grouped_x_box(g.pair, i), chunks,
+                               &maps.x[i])) != TINYM_OK)
+            return st;
+        if (tinym::grouped_x_box(g.pair, i) * (g.pair ? 2 : 1) >= std::min<int64_t>(p.tn, rows)) break;
+    }
     p.y = static_cast<__nv_bfloat16*>(y);
     p.ldy = ldy;
     p.offsets = offsets;
@@ -124,24 +150,29 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
          reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<false, true>)},
         {reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<true, false>),
          reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<true, true>)}};
-    const void* fn = kFn[fp4 ? 1 : 0][g.tile ? 1 : 0];
-    const uint32_t bit = 1u << ((fp4 ? 2 : 0) + (g.tile ? 1 : 0));
+    const void* fn = kFn[fp4 ? 1 : 0][g.pair ? 1 : 0];
+    const uint32_t bit = 1u << ((fp4 ? 2 : 0) + (g.pair ? 1 : 0));
     if (!(g_grouped_attr[dev].load(std::memory_order_acquire) & bit)) {
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");
         g_grouped_attr[dev].fetch_or(bit, std::memory_order_acq_rel);
     }
-    cudaLaunchConfig_t cfg{};
-    cudaLaunchAttribute attr{};
-    cfg.gridDim = dim3(static_cast<unsigned>(g.grid));
-    cfg.blockDim = dim3(tinym::kGrpThreads);
-    cfg.dynamicSmemBytes = g.smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = kUsePdl ? 1 : 0;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    void* args[3] = {&tm_w, &tm_x, &p};
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attrs[2];
+    grouped_config(g, stream, &cfg, attrs);
+    if (g.pair) {
+        // Pairs need two SMs of one cluster: a persistent grid of more pairs
+        // than are resident at once would run its last ones alone.
+        int pairs = g_grouped_pairs[dev].load(std::memory_order_relaxed);
+        if (!pairs) {
+            e = cudaOccupancyMaxActiveClusters(&pairs, fn, &cfg);
+            if (e != cudaSuccess) return cuda_fail(e, "cudaOccupancyMaxActiveClusters");
+            if (pairs < 1) return fail(TINYM_ERR_CUDA, "no CTA pair fits the device");
+            g_grouped_pairs[dev].store(pairs, std::memory_order_relaxed);
+        }
+        if (g.grid > 2 * pairs) cfg.gridDim.x = static_cast<unsigned>(2 * pairs);
+    }
+    void* args[2] = {&maps, &p};
     e = cudaLaunchKernelExC(&cfg, fn, args);
     if (e != cudaSuccess) return cuda_fail(e, "grouped kernel launch");
     return TINYM_OK;

@@ -40,16 +40,18 @@ void tables(const tinym::GroupedParams& p, const std::vector<int>& raw, std::vec
     }
 }
 
-template <bool TILE>
+template <bool PAIR>
 void check_walk(const tinym::GroupedPlan& g, const std::vector<int>& raw) {
     const tinym::GroupedParams& p = g.prm;
     std::vector<int> off, prefix;
     tables(p, raw, &off, &prefix);
-    const int unit = TILE ? 128 : 8;
-    std::vector<std::vector<unsigned char>> seen(p.rows, std::vector<unsigned char>(p.units, 0));
+    const int unit = PAIR ? 256 : 8;
+    const int n_units = (p.n + unit - 1) / unit;
+    const int ctas = PAIR ? g.grid / 2 : g.grid;
+    std::vector<std::vector<unsigned char>> seen(p.rows, std::vector<unsigned char>(n_units, 0));
     int least = 1 << 30, most = 0;
-    for (int b = 0; b < g.grid; ++b) {
-        tinym::GroupedWalk<TILE> walk(p, off.data(), prefix.data(), b, g.grid);
+    for (int b = 0; b < ctas; ++b) {
+        tinym::GroupedWalk<PAIR> walk(p, off.data(), prefix.data(), b, ctas);
         tinym::GroupedPiece w;
         int units = 0;
         while (walk.next(&w)) {
@@ -57,9 +59,15 @@ void check_walk(const tinym::GroupedPlan& g, const std::vector<int>& raw) {
             expect(w.rows >= 1 && w.rows <= p.tn, "rows of a piece", w.rows, p.tn);
             expect(w.row0 >= off[w.e] && w.row0 + w.rows <= off[w.e + 1], "piece inside its group",
                    w.row0, w.rows, w.e);
-            expect(w.h >= unit && w.h <= 128 && w.h % unit == 0 && w.w0 % unit == 0, "W rows", w.w0, w.h);
-            expect(w.w0 >= 0 && w.w0 < p.n && w.w0 + w.h <= p.units * unit, "W range", w.w0, w.h);
-            if (!TILE) expect(w.h <= p.piece_units * 8, "piece fits its stage", w.h, p.piece_units);
+            expect(w.h >= unit && w.h <= std::max(128, unit) && w.h % unit == 0 && w.w0 % unit == 0, "W rows",
+                   w.w0, w.h);
+            expect(w.w0 >= 0 && w.w0 < p.n && w.w0 + w.h <= n_units * unit, "W range", w.w0, w.h);
+            if (!PAIR) expect(w.h <= p.piece_units * 8, "piece fits its stage", w.h, p.piece_units);
+            if (!PAIR && p.blocked) {
+                expect(w.w0 / 128 == (w.w0 + w.h - 1) / 128, "piece inside a block", w.w0, w.h);
+                // the MMA reads from the block's first row, ahead of the stage
+                expect(w.w0 % 128 * 128 <= static_cast<int>(p.w_off), "read before the stage", w.w0, p.w_off);
+            }
             for (int r = 0; r < w.rows; ++r)
                 for (int u = 0; u < w.h / unit; ++u) ++seen[w.row0 + r][w.w0 / unit + u];
             units += w.h / unit;
@@ -67,9 +75,11 @@ void check_walk(const tinym::GroupedPlan& g, const std::vector<int>& raw) {
         least = std::min(least, units);
         most = std::max(most, units);
     }
-    expect(most - least <= 1, "equal shares", least, most);
+    if (!p.part_units) expect(most - least <= 1, "equal shares", least, most);
+    else expect(most <= p.part_units * std::max(1, (prefix[p.experts] * p.units + ctas - 1) / ctas),
+                "shares of parts", least, most);
     for (int r = 0; r < p.rows; ++r)
-        for (int u = 0; u < p.units; ++u)
+        for (int u = 0; u < n_units; ++u)
             expect(seen[r][u] == (r >= off[0] && r < off[p.experts] ? 1 : 0), "computed once", r, u,
                    seen[r][u]);
 }
@@ -78,24 +88,33 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
     const tinym::GroupedParams& p = g.prm;
     expect(g.smem <= limit && p.stages >= 2, "shared memory", g.smem, p.stages);
     expect(p.w_stage % 1024 == 0 && p.x_stage % 1024 == 0, "stage alignment", p.w_stage, p.x_stage);
-    expect(p.sf_off == static_cast<uint32_t>(p.stages * (p.w_stage + p.x_stage)) && p.sf_off % 512 == 0 &&
-               p.sf_stage % 512 == 0,
+    expect(p.sf_off >= static_cast<uint32_t>(p.stages * p.x_stage) && p.sf_off % 512 == 0 && p.sf_stage % 512 == 0,
            "scale ring", p.sf_off, p.sf_stage);
-    expect(p.bar_off >= p.sf_off + p.stages * p.sf_stage && p.bar_off % 8 == 0, "barriers", p.bar_off);
-    expect(p.tab_off >= p.bar_off + 8u * (3 * p.stages + 5) + 8u && p.tab_off % 4 == 0, "tables", p.tab_off);
+    expect(p.w_off >= p.sf_off + p.stages * p.sf_stage && p.w_off % 1024 == 0, "W ring", p.w_off);
+    expect(p.bar_off >= p.w_off + p.stages * p.w_stage && p.bar_off % 8 == 0, "barriers", p.bar_off);
+    expect(p.tab_off >= p.bar_off + 8u * (2 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
+           p.tab_off);
     expect(p.tab_off + 8u * (p.experts + 1) + 1024 <= g.smem, "tables inside", p.tab_off, g.smem);
-    const uint32_t w_read = 128u * 128u * (g.tile ? 1 : 4), x_read = (p.tn + 15) / 16 * 16 * 128u * (g.tile ? 1 : 4);
-    expect((p.stages - 1) * p.w_stage + w_read + 1024 <= g.smem, "W read inside", p.w_stage, g.smem);
-    expect(x_read <= static_cast<uint32_t>(p.x_stage), "X read inside its stage", x_read, p.x_stage);
-    expect(p.tn % 16 == 0 && p.tn >= 16 && p.tn <= 256 && (!g.tile || p.tn % 32 == 0) &&
-               p.tn <= 128 * tinym::grouped_x_scale_blocks(g.tile),
+    const uint32_t chunks = g.pair ? 1 : 4;
+    // every W read is 128 rows of a chunk that starts inside its stage, every
+    // X read at most 8 rows longer than the box
+    expect(p.w_off + p.stages * p.w_stage + (g.pair ? 0 : 128 * 128) + 1024 <= g.smem, "W read inside", p.w_stage,
+           g.smem);
+    expect(p.w_stage == p.piece_units * 8 * 128 * static_cast<int>(chunks), "W stage", p.w_stage);
+    int box = 0;
+    while (box < 4 && tinym::grouped_x_box(g.pair, box) * (g.pair ? 2 : 1) < p.tn) ++box;
+    expect(box < 4 && tinym::grouped_x_box(g.pair, box) * 128 * static_cast<int>(chunks) <= p.x_stage, "X box", box,
+           p.x_stage);
+    expect(p.tn % 16 == 0 && p.tn >= 16 && p.tn <= 256 && (!g.pair || p.tn % 64 == 0) &&
+               p.tn <= 128 * tinym::grouped_x_scale_blocks(g.pair),
            "tile width", p.tn);
-    expect(p.acc_cols >= static_cast<uint32_t>(p.tn) && p.tmem_cols <= 512 && (p.tmem_cols & (p.tmem_cols - 1)) == 0,
+    const uint32_t overlap = p.tn - std::min<uint32_t>(p.tn, p.acc_cols);  // columns of both accumulators
+    expect((overlap == 0 || (g.pair && fp4 && p.acc_cols >= 2 * overlap)) && p.tmem_cols <= 512 && (p.tmem_cols & (p.tmem_cols - 1)) == 0,
            "tensor memory", p.acc_cols, p.tmem_cols);
-    expect((fp4 ? p.sf_col + 2 * tinym::kSfSlotCols : 2 * p.acc_cols) <= p.tmem_cols &&
-               (!fp4 || (p.sf_col >= 2 * p.acc_cols && p.sf_col % 4 == 0)),
+    expect((fp4 ? p.sf_col + 2 * tinym::kSfSlotCols : p.acc_cols + p.tn) <= p.tmem_cols &&
+               (!fp4 || (p.sf_col >= p.acc_cols + p.tn && p.sf_col % 4 == 0)),
            "scale columns", p.sf_col, p.tmem_cols);
-    expect(g.grid >= 1, "grid", g.grid);
+    expect(g.grid >= 1 && (!g.pair || g.grid % 2 == 0), "grid", g.grid);
 }
 
 void check_div() {
@@ -141,7 +160,7 @@ int main() {
                             if (mode == 3) off[i] = std::min(rows, 1 + i / 2);            // spare rows
                             if (mode == 4) off[i] = 0;                                    // no rows
                         }
-                        if (g.tile) check_walk<true>(g, off);
+                        if (g.pair) check_walk<true>(g, off);
                         else check_walk<false>(g, off);
                     }
     // large shapes: the plan alone
