@@ -54,8 +54,9 @@ constexpr int kGrpThreads = 256;     // warp 0 TMA, 1 MMA, 2-3 scales, 4-7 epilo
 constexpr int kGrpMaxExperts = 1024;
 constexpr int kGrpBand = 8;          // row tiles walked together for each W tile (L2 reuse)
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
-constexpr int kGrpBars = 7;          // barriers beside the two per stage
-constexpr int kSfDepth = 4;          // scale copies of a warp in flight, in stages
+constexpr int kGrpBars = 7;          // barriers beside the three per stage
+constexpr int kGrpPairCols = 256;    // X rows of a pair's tile
+constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
 struct GroupedParams {
@@ -77,7 +78,8 @@ struct GroupedParams {
     int32_t stages;
     int32_t chunked;          // stream: one box per unit covers the whole stage
     int32_t w_stage, x_stage, sf_stage;  // bytes
-    uint32_t w_off, sf_off, bar_off, tab_off;  // shared-memory offsets (X ring at 0)
+    uint32_t w_off, sf_off, out_off, bar_off, tab_off;  // shared-memory offsets (X ring at 0)
+    int32_t wide_y;           // Y takes 16-byte stores
     uint32_t tmem_cols, acc_cols, sf_col;
     uint32_t flags;
     uint32_t* err_host;
@@ -222,7 +224,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     // inside a scale block stands that many rows into the MMA's rows.
     const uint32_t front = fp4 && !g.pair ? kTileRows * kBlockK : 0;
     if (g.pair) {
-        p.tn = 256;
+        p.tn = kGrpPairCols;
         p.units = static_cast<int32_t>((n + 2 * kTileRows - 1) / (2 * kTileRows));
         p.piece_units = kBlockUnits;
         p.x_stage = p.tn / 2 * kBlockK;
@@ -270,8 +272,9 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.sf_off = static_cast<uint32_t>(stages * p.x_stage);
         p.w_off = p.sf_off + static_cast<uint32_t>(stages * p.sf_stage);
         p.w_off = (std::max(p.w_off, front) + 1023u) & ~1023u;
-        p.bar_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
-        p.tab_off = p.bar_off + 8u * (2 * stages + kGrpBars) + 8u;
+        p.out_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
+        p.bar_off = p.out_off + (g.pair ? 4 * kOutBytes : 0);
+        p.tab_off = p.bar_off + 8u * (3 * stages + kGrpBars) + 8u;
         // The MMA's 128 W rows of the last chunk end inside the allocation.
         const uint32_t read_end = p.w_off + static_cast<uint32_t>(stages * p.w_stage) + kTileRows * kBlockK;
         return std::max(p.tab_off + tables, g.pair ? 0u : read_end) + 1024u;
@@ -419,12 +422,12 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() {
-    asm volatile("cp.async.commit_group;" ::: "memory");
+// This thread's arrival on `bar` once its copies so far have landed.
+__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
 }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+__device__ __forceinline__ void cp_async_wait_all() {
+    asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
 __device__ __forceinline__ void tmem_ld_x16_nowait(uint32_t taddr, uint32_t* r) {
@@ -435,6 +438,31 @@ __device__ __forceinline__ void tmem_ld_x16_nowait(uint32_t taddr, uint32_t* r) 
           "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
           "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(taddr));
+}
+// 16 lanes x 32 columns as the fragments of 8 x 8 matrices: for columns 8 j ..
+// r[4 j], r[4 j + 1] are lane t / 4, columns 2 (t % 4) and + 1, the next two
+// lane t / 4 + 8.
+__device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
+          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+// Four 8 x 8 matrices of 16-bit values, transposed, to the row addresses that
+// lanes 0-7, 8-15, 16-23 and 24-31 give.
+__device__ __forceinline__ void stmatrix_x4_trans(uint32_t addr, uint32_t a, uint32_t b, uint32_t c,
+                                                  uint32_t d) {
+    asm volatile("stmatrix.sync.aligned.m8n8.x4.trans.shared.b16 [%0], {%1, %2, %3, %4};" ::"r"(addr),
+                 "r"(a), "r"(b), "r"(c), "r"(d)
+                 : "memory");
+}
+__device__ __forceinline__ uint32_t pack_bf16(uint32_t lo, uint32_t hi, float alpha) {
+    const __nv_bfloat162 h =
+        __floats2bfloat162_rn(__uint_as_float(lo) * alpha, __uint_as_float(hi) * alpha);
+    return *reinterpret_cast<const uint32_t*>(&h);
 }
 __device__ __forceinline__ void tmem_ld_wait() {
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
@@ -503,11 +531,12 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const uint32_t bars = s_base + p.bar_off;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
-    auto acc_full = [&](int b) { return bars + 8u * (2 * stages + b); };
-    auto acc_empty = [&](int b) { return bars + 8u * (2 * stages + 2 + b); };
-    auto acc_part = [&](int b) { return bars + 8u * (2 * stages + 4 + b); };
-    const uint32_t drain_bar = bars + 8u * (2 * stages + 6);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (2 * stages + kGrpBars));
+    auto sf_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
+    auto acc_full = [&](int b) { return bars + 8u * (3 * stages + b); };
+    auto acc_empty = [&](int b) { return bars + 8u * (3 * stages + 2 + b); };
+    auto acc_part = [&](int b) { return bars + 8u * (3 * stages + 4 + b); };
+    const uint32_t drain_bar = bars + 8u * (3 * stages + 6);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (3 * stages + kGrpBars));
     volatile uint32_t* abort_flag = tmem_slot + 1;
     int32_t* off = reinterpret_cast<int32_t*>(smem + p.tab_off);
     int32_t* prefix = off + p.experts + 1;
@@ -522,10 +551,11 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            // full: the producer's expect_tx (and the bytes), the two scale
-            // warps, and at CTA 0 of a pair the stage of CTA 1
-            mbar_init(full_bar(s), 1 + (FP4 ? 2 : 0) + (PAIR && rank == 0 ? 1 : 0));
+            // full: the producer's expect_tx (and the bytes), the scales, and
+            // at CTA 0 of a pair the stage of CTA 1
+            mbar_init(full_bar(s), 1 + (FP4 ? 1 : 0) + (PAIR && rank == 0 ? 1 : 0));
             mbar_init(empty_bar(s), 1);
+            mbar_init(sf_bar(s), 32);  // the lanes of the scale warp
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
@@ -731,100 +761,105 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             }
         }
     } else if (warp < 4) {
-        // ---------------- MXFP4 scales.  Warps 2 and 3 take alternate blocks of
-        // K: a block of W as it lies in memory (one 16-byte copy per lane), X
-        // rows as 4-byte words gathered into the block order.
+        // ---------------- MXFP4 scales.  Warp 2 copies them: a block of W as it
+        // lies in memory (one 16-byte copy per lane), X rows as 4-byte words
+        // gathered into the block order.  It never waits for a copy: their
+        // completion arrives on sf_bar, where warp 3 waits, makes them visible
+        // to the tensor core's copies and passes them on.
         if constexpr (FP4) {
-            const int blocks = (p.k_bytes * 2 + 127) / 128;     // scale blocks along K
-            const int tail = (p.k_bytes * 2 % 128) / 32;        // scales in the last one, 0: all
-            const uint32_t tail_mask = tail ? (1u << (8 * tail)) - 1u : 0xFFFFFFFFu;
-            int s = 0, pending = 0, ps = 0;
-            uint32_t ph = 1u;
+            int s = 0;
             bool ok = true;
-            auto arrive = [&]() {  // the oldest pending stage
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(full_bar(ps));
-                if (++ps == stages) ps = 0;
-                --pending;
-            };
-            auto flush = [&]() {
-                cp_async_wait<0>();
-                while (pending > 0) arrive();
-            };
-            while (ok && walk.next(&w)) {
-                const int w0 = w.w0 + rank * kTileRows;
-                const uint8_t* ws = p.w_scales + w.e * p.w_scale_stride +
-                                    static_cast<int64_t>(w0 >> 7) * blocks * kScaleBlock + lane * 16;
-                const bool w_in = w0 < p.n;
-                const int x_groups = (w.rows + 31) / 32;
-                for (int i = 0; i < nkb; ++i) {
-                    if (!warp_try<PAIR>(empty_bar(s), ph)) {
-                        flush();  // before blocking: the MMA may need what is pending
-                        ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait);
-                        if (!ok) break;
-                    }
-                    const uint32_t sf = sf_ring + s * p.sf_stage;
-                    const int b0 = i * kChunks * kSfPerChunk;
+            if (warp == 2) {
+                constexpr int kGroups = PAIR ? kGrpPairCols / 32 : 2;  // of 32 X rows
+                const int blocks = (p.k_bytes * 2 + 127) / 128;     // scale blocks along K
+                const int tail = (p.k_bytes * 2 % 128) / 32;        // scales in the last one, 0: all
+                const uint32_t tail_mask = tail ? (1u << (8 * tail)) - 1u : 0xFFFFFFFFu;
+                uint32_t ph = 1u;
+                while (ok && walk.next(&w)) {
+                    const int w0 = w.w0 + rank * kTileRows;
+                    const bool w_in = w0 < p.n;
+                    const uint8_t* ws = p.w_scales + w.e * p.w_scale_stride +
+                                        static_cast<int64_t>(w0 >> 7) * blocks * kScaleBlock + lane * 16;
+                    const uint8_t* xs[kGroups];
 #pragma unroll
-                    for (int j = 0; j < kChunks * kSfPerChunk / 2; ++j) {
-                        const int q = 2 * j + warp - 2;
-                        const int kb = b0 + q;
-                        const uint32_t wd = sf + q * kScaleBlock + lane * 16;
-                        const uint32_t xd = sf + kWsBytes + q * kXsBlocks * kScaleBlock + lane * 16;
-                        if (kb < blocks - 1 || (kb == blocks - 1 && !tail)) {
-                            if (w_in) cp_async_16(wd, ws + static_cast<int64_t>(kb) * kScaleBlock);
-                            for (int g = 0; g < x_groups; ++g) {
-                                const int r = w.row0 + min(g * 32 + lane, w.rows - 1);
-                                cp_async_4(xd + (g >> 2) * kScaleBlock + (g & 3) * 4,
-                                           p.x_scales +
-                                               (static_cast<int64_t>(r >> 7) * blocks + kb) * kScaleBlock +
-                                               (r & 31) * 16 + ((r >> 5) & 3) * 4);
+                    for (int g = 0; g < kGroups; ++g) {
+                        const int r = w.row0 + min(g * 32 + lane, w.rows - 1);
+                        xs[g] = p.x_scales + static_cast<int64_t>(r >> 7) * blocks * kScaleBlock +
+                                (r & 31) * 16 + ((r >> 5) & 3) * 4;
+                    }
+                    for (int i = 0; i < nkb; ++i) {
+                        if (!(ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait))) break;
+                        const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
+                        const uint32_t xd = wd + kWsBytes;
+                        const int b0 = i * kChunks * kSfPerChunk;
+                        const bool whole = b0 + kChunks * kSfPerChunk < blocks + (tail == 0 ? 1 : 0);
+                        if (whole) {
+#pragma unroll
+                            for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
+                                const int64_t at = static_cast<int64_t>(b0 + q) * kScaleBlock;
+                                if (w_in) cp_async_16(wd + q * kScaleBlock, ws + at);
+#pragma unroll
+                                for (int g = 0; g < kGroups; ++g)
+                                    if (g * 32 < w.rows)
+                                        cp_async_4(xd + (q * kXsBlocks + (g >> 2)) * kScaleBlock + (g & 3) * 4,
+                                                   xs[g] + at);
                             }
+                            cp_async_arrive(sf_bar(s));
                         } else {
-                            // The last, partial block: scales past K become 2^-127
-                            // (the data there are zeros); a block past K likewise.
-                            const uint32_t mask = kb < blocks ? tail_mask : 0u;
-                            const int kc = min(kb, blocks - 1);
-                            if (w_in) {
-                                const uint4 v = __ldg(reinterpret_cast<const uint4*>(
-                                    ws + static_cast<int64_t>(kc) * kScaleBlock));
-                                asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(wd),
-                                             "r"(v.x & mask), "r"(v.y & mask), "r"(v.z & mask),
-                                             "r"(v.w & mask)
-                                             : "memory");
+                            // The last stage: scales past K become 2^-127 (the data
+                            // there are zeros), blocks past K likewise.
+                            for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
+                                const uint32_t mask = b0 + q < blocks - 1 ? 0xFFFFFFFFu
+                                                      : b0 + q < blocks   ? tail_mask : 0u;
+                                const int64_t at = static_cast<int64_t>(min(b0 + q, blocks - 1)) * kScaleBlock;
+                                if (w_in) {
+                                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(ws + at));
+                                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
+                                                     wd + q * kScaleBlock),
+                                                 "r"(v.x & mask), "r"(v.y & mask), "r"(v.z & mask),
+                                                 "r"(v.w & mask)
+                                                 : "memory");
+                                }
+#pragma unroll
+                                for (int g = 0; g < kGroups; ++g)
+                                    if (g * 32 < w.rows) {
+                                        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(xs[g] + at));
+                                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(
+                                                         xd + (q * kXsBlocks + (g >> 2)) * kScaleBlock + (g & 3) * 4),
+                                                     "r"(v & mask)
+                                                     : "memory");
+                                    }
                             }
-                            for (int g = 0; g < x_groups; ++g) {
-                                const int r = w.row0 + min(g * 32 + lane, w.rows - 1);
-                                const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(
-                                    p.x_scales +
-                                    (static_cast<int64_t>(r >> 7) * blocks + kc) * kScaleBlock +
-                                    (r & 31) * 16 + ((r >> 5) & 3) * 4));
-                                asm volatile("st.shared.u32 [%0], %1;" ::"r"(
-                                                 xd + (g >> 2) * kScaleBlock + (g & 3) * 4),
-                                             "r"(v & mask)
-                                             : "memory");
-                            }
+                            mbar_arrive(sf_bar(s));
+                        }
+                        if (++s == stages) {
+                            s = 0;
+                            ph ^= 1u;
                         }
                     }
-                    cp_async_commit();
-                    if (++pending == kSfDepth) {
-                        cp_async_wait<kSfDepth - 1>();
-                        arrive();
-                    }
-                    if (++s == stages) {
-                        s = 0;
-                        ph ^= 1u;
+                }
+                cp_async_wait_all();  // none is in flight when shared memory is released
+            } else {
+                uint32_t ph = 0u;
+                while (ok && walk.next(&w)) {
+                    for (int i = 0; i < nkb; ++i) {
+                        if (!(ok = warp_wait(sf_bar(s), ph, guard, kErrConsumerWait))) break;
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (elect_one()) mbar_arrive(full_bar(s));
+                        __syncwarp();
+                        if (++s == stages) {
+                            s = 0;
+                            ph ^= 1u;
+                        }
                     }
                 }
             }
-            flush();
         }
     } else {
         // ---------------- epilogue: warp w reads TMEM lanes 32 (w % 4) ..
         const int q = warp & 3;
         int piece = 0;
-        constexpr int kCols = PAIR ? 32 : 16;
         while (walk.next(&w)) {
             const int b = piece & 1;
             if (!warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait)) break;
@@ -833,43 +868,96 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                 mbar_arrive_remote(at_rank(acc_full(b), 1));
             tc_fence_after_sync();
             const float alpha = p.alpha ? __ldg(p.alpha + w.e * p.alpha_stride) : 1.0f;
-            const int r = q * 32 + lane - first_row();  // W row of the piece
-            const int n = w.w0 + rank * kTileRows + r;
-            const bool mine = r >= 0 && r < (PAIR ? kTileRows : w.h) && n < p.n;
-            __nv_bfloat16* dst = p.y + static_cast<int64_t>(w.row0) * p.ldy + n;
             const uint32_t taddr = tmem + b * p.acc_cols + (static_cast<uint32_t>(q * 32) << 16);
-            // Columns that both accumulators use come first: the upper ones of
-            // buffer 0, the lower ones of buffer 1.
-            const int cols = (w.rows + kCols - 1) / kCols;
-            const int shared_cols = static_cast<int>(256 - p.acc_cols) / kCols;
-            const int start = PAIR && FP4 && b == 0 && cols * kCols > static_cast<int>(p.acc_cols)
-                                  ? static_cast<int>(p.acc_cols) / kCols : 0;
-            for (int j = 0; j < cols; ++j) {
-                const int c = (j + start < cols ? j + start : j + start - cols) * kCols;
-                uint32_t v[kCols];
+            __nv_bfloat16* row0 = p.y + static_cast<int64_t>(w.row0) * p.ldy;
+            if constexpr (PAIR) {
+                const int n0 = w.w0 + rank * kTileRows + q * 32;  // this warp's first W row
+                // Columns that both accumulators use come first: the upper
+                // ones of buffer 0, the lower ones of buffer 1.
+                const int cols = (w.rows + 31) / 32;
+                const int own = static_cast<int>(p.acc_cols) / 32;
+                const int shared_cols = kGrpPairCols / 32 - own;
+                const int start = FP4 && b == 0 && cols > own ? own : 0;
+                // 32 X rows at a time through shared memory, [X row][32 W rows]
+                // of BF16 with the 16-byte chunks of a row exchanged so that
+                // neither side has bank conflicts.
+                uint8_t* buf = smem + p.out_off + q * kOutBytes;
+                for (int j = 0; j < cols; ++j) {
+                    const int c = (j + start < cols ? j + start : j + start - cols) * 32;
+                    uint32_t v[2][16];
+                    tmem_ld_frag(taddr + c, v[0]);
+                    tmem_ld_frag(taddr + (16u << 16) + c, v[1]);
+                    tmem_ld_wait();
+                    if (FP4 && j == min(shared_cols, cols) - 1) {
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (rank) mbar_arrive_remote(at_rank(acc_part(b), 0));
+                            else mbar_arrive(acc_part(b));
+                        }
+                    }
+                    if (j == cols - 1) {  // everything is read: the accumulator is free
+                        tc_fence_before_sync();
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (rank) mbar_arrive_remote(at_rank(acc_empty(b), 0));
+                            else mbar_arrive(acc_empty(b));
+                        }
+                    }
+                    if (n0 >= p.n) continue;
 #pragma unroll
-                for (int h = 0; h < kCols; h += 16) tmem_ld_x16_nowait(taddr + c + h, v + h);
-                tmem_ld_wait();
-                if (PAIR && FP4 && j == min(shared_cols, cols) - 1) {
-                    tc_fence_before_sync();
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int g = 0; g < 4; g += 2) {
+                            const int r = 8 * (g + (lane >> 4)) + (lane & 7);
+                            const int ch = 2 * h + ((lane >> 3) & 1);
+                            const uint32_t* f = v[h] + 4 * g;
+                            stmatrix_x4_trans(smem_u32(buf) + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16),
+                                              pack_bf16(f[0], f[1], alpha), pack_bf16(f[2], f[3], alpha),
+                                              pack_bf16(f[4], f[5], alpha), pack_bf16(f[6], f[7], alpha));
+                        }
                     __syncwarp();
-                    if (lane == 0) {
-                        if (rank) mbar_arrive_remote(at_rank(acc_part(b), 0));
-                        else mbar_arrive(acc_part(b));
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int r = 8 * k + (lane >> 2), ch = lane & 3;
+                        const int n = n0 + ch * 8;
+                        const uint4 o = *reinterpret_cast<const uint4*>(
+                            buf + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16));
+                        if (c + r < w.rows && n < p.n) {
+                            __nv_bfloat16* dst = row0 + (c + r) * p.ldy + n;
+                            if (p.wide_y && n + 8 <= p.n) {
+                                *reinterpret_cast<uint4*>(dst) = o;
+                            } else {
+                                const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                                for (int i = 0; i < 8; ++i)
+                                    if (n + i < p.n)
+                                        reinterpret_cast<uint16_t*>(dst)[i] =
+                                            static_cast<uint16_t>(ow[i / 2] >> (16 * (i & 1)));
+                            }
+                        }
+                    }
+                    __syncwarp();
+                }
+            } else {
+                const int r = q * 32 + lane - first_row();  // W row of the piece
+                const int n = w.w0 + r;
+                const bool mine = r >= 0 && r < w.h && n < p.n;
+                for (int c = 0; c < w.rows; c += 16) {
+                    uint32_t v[16];
+                    tmem_ld_x16_nowait(taddr + c, v);
+                    tmem_ld_wait();
+                    if (mine) {
+#pragma unroll
+                        for (int h = 0; h < 16; ++h)
+                            if (c + h < w.rows)
+                                row0[(c + h) * p.ldy + n] =
+                                    __float2bfloat16_rn(__uint_as_float(v[h]) * alpha);
                     }
                 }
-                if (mine) {
-#pragma unroll
-                    for (int h = 0; h < kCols; ++h)
-                        if (c + h < w.rows)
-                            dst[(c + h) * p.ldy] = __float2bfloat16_rn(__uint_as_float(v[h]) * alpha);
-                }
-            }
-            tc_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                if (PAIR && rank) mbar_arrive_remote(at_rank(acc_empty(b), 0));
-                else mbar_arrive(acc_empty(b));
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty(b));
             }
             ++piece;
         }

@@ -134,6 +134,7 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
     }
     p.y = static_cast<__nv_bfloat16*>(y);
     p.ldy = ldy;
+    p.wide_y = ldy % 8 == 0 && (reinterpret_cast<uintptr_t>(y) & 15u) == 0;
     p.offsets = offsets;
     p.alpha = alpha;
     p.alpha_stride = alpha_count > 1 ? 1 : 0;

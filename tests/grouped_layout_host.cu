@@ -91,8 +91,9 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
     expect(p.sf_off >= static_cast<uint32_t>(p.stages * p.x_stage) && p.sf_off % 512 == 0 && p.sf_stage % 512 == 0,
            "scale ring", p.sf_off, p.sf_stage);
     expect(p.w_off >= p.sf_off + p.stages * p.sf_stage && p.w_off % 1024 == 0, "W ring", p.w_off);
-    expect(p.bar_off >= p.w_off + p.stages * p.w_stage && p.bar_off % 8 == 0, "barriers", p.bar_off);
-    expect(p.tab_off >= p.bar_off + 8u * (2 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
+    expect(p.out_off >= p.w_off + p.stages * p.w_stage && p.out_off % 16 == 0, "output", p.out_off);
+    expect(p.bar_off >= p.out_off + (g.pair ? 4u * tinym::kOutBytes : 0u) && p.bar_off % 8 == 0, "barriers", p.bar_off);
+    expect(p.tab_off >= p.bar_off + 8u * (3 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
            p.tab_off);
     expect(p.tab_off + 8u * (p.experts + 1) + 1024 <= g.smem, "tables inside", p.tab_off, g.smem);
     const uint32_t chunks = g.pair ? 1 : 4;
