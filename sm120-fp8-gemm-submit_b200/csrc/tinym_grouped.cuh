@@ -54,8 +54,7 @@ constexpr int kGrpThreads = 256;     // warp 0 TMA, 1 MMA, 2-3 scales, 4-7 epilo
 constexpr int kGrpMaxExperts = 1024;
 constexpr int kGrpBand = 8;          // row tiles walked together for each W tile (L2 reuse)
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
-constexpr int kGrpBars = 7;          // barriers beside the three per stage
-constexpr int kGrpPairCols = 256;    // X rows of a pair's tile
+constexpr int kGrpBars = 5;          // barriers beside the three per stage
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
@@ -194,6 +193,29 @@ struct GroupedWalk {
     }
 };
 
+// A walk that works out the next piece ahead of time (several integer
+// divisions, ~1,000 cycles), while a role has nothing urgent to do.
+template <bool PAIR>
+struct GroupedAhead {
+    GroupedWalk<PAIR> walk;
+    GroupedPiece nx;
+    bool have, more;
+
+    __device__ __forceinline__ GroupedAhead(const GroupedParams& p, const int32_t* o,
+                                            const int32_t* pre, int block, int blocks)
+        : walk(p, o, pre, block, blocks), have(false), more(false) {}
+    __device__ __forceinline__ void ahead() {
+        if (!have) more = walk.next(&nx);
+        have = true;
+    }
+    __device__ __forceinline__ bool next(GroupedPiece* w) {
+        ahead();
+        have = false;
+        *w = nx;
+        return more;
+    }
+};
+
 // How a call is cut.
 struct GroupedPlan {
     bool pair;
@@ -224,14 +246,14 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     // inside a scale block stands that many rows into the MMA's rows.
     const uint32_t front = fp4 && !g.pair ? kTileRows * kBlockK : 0;
     if (g.pair) {
-        p.tn = kGrpPairCols;
         p.units = static_cast<int32_t>((n + 2 * kTileRows - 1) / (2 * kTileRows));
         p.piece_units = kBlockUnits;
-        p.x_stage = p.tn / 2 * kBlockK;
-        // Two accumulators.  With the scales' 64 columns there is no room for
-        // two of 256: the second starts at column 192, and the epilogue
-        // empties the 64 columns that both use first.
-        p.acc_cols = fp4 ? 192 : 256;
+        // Two accumulators, so that a tile is stored while the next one is
+        // computed; the scales take 64 of the 512 columns.  (Two of 256 that
+        // share 64 columns cost ~2,600 cycles a tile until those are free.)
+        p.tn = fp4 ? 224 : 256;
+        p.acc_cols = static_cast<uint32_t>(p.tn);
+        p.x_stage = kTileRows * kBlockK;
         p.sf_col = 448;
         p.tmem_cols = 512;
     } else {
@@ -422,6 +444,26 @@ __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
+// A lane's 16 bytes of the scale blocks of one pair stage.
+struct ScaleRegs {
+    uint4 w[2], x[2][3];
+    int rot, block;
+    bool valid;
+};
+// Words rot .. rot + 3 of the eight words a, b (rot <= 4).
+__device__ __forceinline__ uint4 rotate_words(const uint4& a, const uint4& b, int rot) {
+    uint32_t v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+    for (int k = 4; k >= 1; k /= 2)
+#pragma unroll
+        for (int j = 0; j + k < 8; ++j) v[j] = rot & k ? v[j + k] : v[j];
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+__device__ __forceinline__ void sts_masked(uint32_t dst, const uint4& v, uint32_t mask) {
+    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(dst), "r"(v.x & mask),
+                 "r"(v.y & mask), "r"(v.z & mask), "r"(v.w & mask)
+                 : "memory");
+}
 // This thread's arrival on `bar` once its copies so far have landed.
 __device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
@@ -534,8 +576,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     auto sf_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
     auto acc_full = [&](int b) { return bars + 8u * (3 * stages + b); };
     auto acc_empty = [&](int b) { return bars + 8u * (3 * stages + 2 + b); };
-    auto acc_part = [&](int b) { return bars + 8u * (3 * stages + 4 + b); };
-    const uint32_t drain_bar = bars + 8u * (3 * stages + 6);
+    const uint32_t drain_bar = bars + 8u * (3 * stages + 4);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (3 * stages + kGrpBars));
     volatile uint32_t* abort_flag = tmem_slot + 1;
     int32_t* off = reinterpret_cast<int32_t*>(smem + p.tab_off);
@@ -560,7 +601,6 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
             mbar_init(acc_empty(b), 4 * kCtas);  // one arrival per epilogue warp
-            mbar_init(acc_part(b), 4 * kCtas);
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0u;
@@ -582,7 +622,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     tc_fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    GroupedWalk<PAIR> walk(p, off, prefix, blockIdx.x / kCtas, gridDim.x / kCtas);
+    GroupedAhead<PAIR> walk(p, off, prefix, blockIdx.x / kCtas, gridDim.x / kCtas);
     GroupedPiece w;
     // MMA row of a stream piece's first W row (0 unless scales are blocked).
     auto first_row = [&]() { return !PAIR && FP4 ? w.w0 % kTileRows : 0; };
@@ -639,6 +679,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                     }
                 }
                 __syncwarp();
+                if (i == 0) walk.ahead();
                 ++issued;
                 if (++s == stages) {
                     s = 0;
@@ -659,7 +700,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             const uint32_t tmem_u = __shfl_sync(0xFFFFFFFFu, tmem, 0);
             const uint64_t da0 = sw128_kmajor_desc(w_ring);
             const uint64_t db0 = sw128_kmajor_desc(x_ring);
-            int s = 0, piece = 0, slot = 0, last_cols = 0;
+            int s = 0, piece = 0, slot = 0;
             uint32_t ph = 0u;
             bool ok = true;
             while (ok && walk.next(&w)) {
@@ -669,14 +710,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                                            : idesc_e4m3_f32(kCtas * 128, mma_n);
                 const uint32_t acc = tmem_u + b * p.acc_cols;
                 const bool two = PAIR && mma_n > 128;  // X scale blocks of the tile
-                // The piece's own accumulator is free, and so are the columns
-                // that it shares with the one before.
-                const int lower = b ? last_cols : static_cast<int>(mma_n);  // columns used of buffer 0
-                ok = warp_wait<PAIR>(acc_empty(b), ((piece >> 1) & 1) ^ 1u, guard, kErrMmaWait);
-                if (PAIR && FP4 && ok && piece > 0 && lower > static_cast<int>(p.acc_cols))
-                    ok = warp_wait<PAIR>(acc_part(b ^ 1), ((piece - 1) >> 1) & 1, guard, kErrMmaWait);
-                if (!ok) break;
-                last_cols = mma_n;
+                if (!(ok = warp_wait<PAIR>(acc_empty(b), ((piece >> 1) & 1) ^ 1u, guard, kErrMmaWait)))
+                    break;
                 tc_fence_after_sync();
                 // Bytes from chunk to chunk of a stage, and of the rows that
                 // stand in front of a blocked piece's first one.
@@ -728,6 +763,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                         if (i == nkb - 1) Ops::commit(acc_full(b));
                     }
                     __syncwarp();
+                    if (i == 0) walk.ahead();
                     slot += kChunks;
                     if (++s == stages) {
                         s = 0;
@@ -753,6 +789,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                     if (!(ok = warp_wait(full_bar(s), ph, guard, kErrMmaWait))) break;
                     if (elect_one()) mbar_arrive_remote(at_rank(full_bar(s), 0));
                     __syncwarp();
+                    if (i == 0) walk.ahead();
                     if (++s == stages) {
                         s = 0;
                         ph ^= 1u;
@@ -761,25 +798,105 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             }
         }
     } else if (warp < 4) {
-        // ---------------- MXFP4 scales.  Warp 2 copies them: a block of W as it
-        // lies in memory (one 16-byte copy per lane), X rows as 4-byte words
-        // gathered into the block order.  It never waits for a copy: their
-        // completion arrives on sf_bar, where warp 3 waits, makes them visible
-        // to the tensor core's copies and passes them on.
-        if constexpr (FP4) {
+        // ---------------- MXFP4 scales
+        const int blocks = (p.k_bytes * 2 + 127) / 128;  // scale blocks along K
+        const int tail = (p.k_bytes * 2 % 128) / 32;     // scales in the last one, 0: all
+        const uint32_t tail_mask = tail ? (1u << (8 * tail)) - 1u : 0xFFFFFFFFu;
+        // Scales past K become 2^-127 (the data there are zeros).
+        auto block_mask = [&](int b) {
+            return b < blocks - 1 ? 0xFFFFFFFFu : b < blocks ? tail_mask : 0u;
+        };
+        if constexpr (FP4 && PAIR) {
+            // Warps 2 and 3 take alternate stages, each with the scales of its
+            // next two in registers: a stage's are stored when its slot is
+            // free, and those of four stages later loaded.  A W block is
+            // stored as it is.  An X tile that starts at row r0 of the blocks
+            // needs from lane i the words of rows r0 + 32 j + i: those of
+            // block row (i + r0) % 32, rotated, from two or three blocks.
+            // (Words copied one by one, by cp.async, took ~900 cycles a stage.)
+            ScaleRegs ra, rb;
+            const uint8_t *ws = nullptr, *xs[3] = {nullptr, nullptr, nullptr};
+            int i = warp - 2, rot = 0;
+            auto enter = [&]() {  // a piece
+                const int w0 = min(w.w0 + rank * kTileRows, p.n - 1);
+                ws = p.w_scales + w.e * p.w_scale_stride +
+                     static_cast<int64_t>(w0 >> 7) * blocks * kScaleBlock + lane * 16;
+                const int first = w.row0 >> 7, last = (w.row0 + w.rows - 1) >> 7;
+                const int src = lane + (w.row0 & 31);
+                rot = ((w.row0 & 127) >> 5) + (src >> 5);
+#pragma unroll
+                for (int j = 0; j < 3; ++j)
+                    xs[j] = p.x_scales + static_cast<int64_t>(min(first + j, last)) * blocks * kScaleBlock +
+                            (src & 31) * 16;
+            };
+            auto load = [&](ScaleRegs* r) {
+                r->rot = rot;
+                r->block = i * kSfPerChunk;
+#pragma unroll
+                for (int q = 0; q < kSfPerChunk; ++q) {
+                    const int64_t at = static_cast<int64_t>(min(r->block + q, blocks - 1)) * kScaleBlock;
+                    r->w[q] = __ldg(reinterpret_cast<const uint4*>(ws + at));
+#pragma unroll
+                    for (int j = 0; j < 3; ++j)
+                        r->x[q][j] = __ldg(reinterpret_cast<const uint4*>(xs[j] + at));
+                }
+            };
+            bool more = walk.next(&w);
+            if (more) enter();
+            auto fetch = [&](ScaleRegs* r) {  // this warp's next stage, if there is one
+                while (more && i >= nkb) {
+                    i -= nkb;
+                    if ((more = walk.next(&w))) enter();
+                }
+                r->valid = more;
+                if (more) load(r);
+                i += 2;
+            };
+            fetch(&ra);
+            fetch(&rb);
+            int s = warp - 2;
+            uint32_t ph = 1u;
+            auto step = [&](ScaleRegs& r) {
+                if (!r.valid || !warp_wait<true>(empty_bar(s), ph, guard, kErrProducerWait)) return false;
+                const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
+                const uint32_t xd = wd + kWsBytes;
+#pragma unroll
+                for (int q = 0; q < kSfPerChunk; ++q) {
+                    const uint32_t mask = block_mask(r.block + q);
+                    sts_masked(wd + q * kScaleBlock, r.w[q], mask);
+                    sts_masked(xd + q * kXsBlocks * kScaleBlock,
+                               rotate_words(r.x[q][0], r.x[q][1], r.rot), mask);
+                    sts_masked(xd + (q * kXsBlocks + 1) * kScaleBlock,
+                               rotate_words(r.x[q][1], r.x[q][2], r.rot), mask);
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(full_bar(s));
+                __syncwarp();
+                if ((s += 2) >= stages) {
+                    s -= stages;
+                    ph ^= 1u;
+                }
+                fetch(&r);
+                return true;
+            };
+            while (step(ra) && step(rb)) {
+            }
+        }
+        if constexpr (FP4 && !PAIR) {
+            // Warp 2 copies them: a block of W as it lies in memory (one
+            // 16-byte copy per lane), X rows as 4-byte words gathered into the
+            // block order.  It never waits for a copy: their completion arrives
+            // on sf_bar, where warp 3 waits, makes them visible to the tensor
+            // core's copies and passes them on.
             int s = 0;
             bool ok = true;
             if (warp == 2) {
-                constexpr int kGroups = PAIR ? kGrpPairCols / 32 : 2;  // of 32 X rows
-                const int blocks = (p.k_bytes * 2 + 127) / 128;     // scale blocks along K
-                const int tail = (p.k_bytes * 2 % 128) / 32;        // scales in the last one, 0: all
-                const uint32_t tail_mask = tail ? (1u << (8 * tail)) - 1u : 0xFFFFFFFFu;
+                constexpr int kGroups = 2;  // of 32 X rows
                 uint32_t ph = 1u;
                 while (ok && walk.next(&w)) {
-                    const int w0 = w.w0 + rank * kTileRows;
-                    const bool w_in = w0 < p.n;
                     const uint8_t* ws = p.w_scales + w.e * p.w_scale_stride +
-                                        static_cast<int64_t>(w0 >> 7) * blocks * kScaleBlock + lane * 16;
+                                        static_cast<int64_t>(w.w0 >> 7) * blocks * kScaleBlock + lane * 16;
                     const uint8_t* xs[kGroups];
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
@@ -788,7 +905,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                                 (r & 31) * 16 + ((r >> 5) & 3) * 4;
                     }
                     for (int i = 0; i < nkb; ++i) {
-                        if (!(ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait))) break;
+                        if (!(ok = warp_wait(empty_bar(s), ph, guard, kErrProducerWait))) break;
                         const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
                         const uint32_t xd = wd + kWsBytes;
                         const int b0 = i * kChunks * kSfPerChunk;
@@ -797,35 +914,24 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
 #pragma unroll
                             for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
                                 const int64_t at = static_cast<int64_t>(b0 + q) * kScaleBlock;
-                                if (w_in) cp_async_16(wd + q * kScaleBlock, ws + at);
+                                cp_async_16(wd + q * kScaleBlock, ws + at);
 #pragma unroll
                                 for (int g = 0; g < kGroups; ++g)
                                     if (g * 32 < w.rows)
-                                        cp_async_4(xd + (q * kXsBlocks + (g >> 2)) * kScaleBlock + (g & 3) * 4,
-                                                   xs[g] + at);
+                                        cp_async_4(xd + q * kScaleBlock + g * 4, xs[g] + at);
                             }
                             cp_async_arrive(sf_bar(s));
                         } else {
-                            // The last stage: scales past K become 2^-127 (the data
-                            // there are zeros), blocks past K likewise.
                             for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
-                                const uint32_t mask = b0 + q < blocks - 1 ? 0xFFFFFFFFu
-                                                      : b0 + q < blocks   ? tail_mask : 0u;
+                                const uint32_t mask = block_mask(b0 + q);
                                 const int64_t at = static_cast<int64_t>(min(b0 + q, blocks - 1)) * kScaleBlock;
-                                if (w_in) {
-                                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(ws + at));
-                                    asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(
-                                                     wd + q * kScaleBlock),
-                                                 "r"(v.x & mask), "r"(v.y & mask), "r"(v.z & mask),
-                                                 "r"(v.w & mask)
-                                                 : "memory");
-                                }
+                                sts_masked(wd + q * kScaleBlock, __ldg(reinterpret_cast<const uint4*>(ws + at)),
+                                           mask);
 #pragma unroll
                                 for (int g = 0; g < kGroups; ++g)
                                     if (g * 32 < w.rows) {
                                         const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(xs[g] + at));
-                                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(
-                                                         xd + (q * kXsBlocks + (g >> 2)) * kScaleBlock + (g & 3) * 4),
+                                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(xd + q * kScaleBlock + g * 4),
                                                      "r"(v & mask)
                                                      : "memory");
                                     }
@@ -862,6 +968,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         int piece = 0;
         while (walk.next(&w)) {
             const int b = piece & 1;
+            walk.ahead();
             if (!warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait)) break;
             // The MMAs' commit reaches CTA 0 alone: pass it on.
             if (PAIR && rank == 0 && warp == 4 && lane == 0)
@@ -872,31 +979,16 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             __nv_bfloat16* row0 = p.y + static_cast<int64_t>(w.row0) * p.ldy;
             if constexpr (PAIR) {
                 const int n0 = w.w0 + rank * kTileRows + q * 32;  // this warp's first W row
-                // Columns that both accumulators use come first: the upper
-                // ones of buffer 0, the lower ones of buffer 1.
-                const int cols = (w.rows + 31) / 32;
-                const int own = static_cast<int>(p.acc_cols) / 32;
-                const int shared_cols = kGrpPairCols / 32 - own;
-                const int start = FP4 && b == 0 && cols > own ? own : 0;
                 // 32 X rows at a time through shared memory, [X row][32 W rows]
                 // of BF16 with the 16-byte chunks of a row exchanged so that
                 // neither side has bank conflicts.
                 uint8_t* buf = smem + p.out_off + q * kOutBytes;
-                for (int j = 0; j < cols; ++j) {
-                    const int c = (j + start < cols ? j + start : j + start - cols) * 32;
+                for (int c = 0; c < w.rows; c += 32) {
                     uint32_t v[2][16];
                     tmem_ld_frag(taddr + c, v[0]);
                     tmem_ld_frag(taddr + (16u << 16) + c, v[1]);
                     tmem_ld_wait();
-                    if (FP4 && j == min(shared_cols, cols) - 1) {
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (rank) mbar_arrive_remote(at_rank(acc_part(b), 0));
-                            else mbar_arrive(acc_part(b));
-                        }
-                    }
-                    if (j == cols - 1) {  // everything is read: the accumulator is free
+                    if (c + 32 >= w.rows) {  // everything is read: the accumulator is free
                         tc_fence_before_sync();
                         __syncwarp();
                         if (lane == 0) {

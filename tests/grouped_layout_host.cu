@@ -106,11 +106,10 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
     while (box < 4 && tinym::grouped_x_box(g.pair, box) * (g.pair ? 2 : 1) < p.tn) ++box;
     expect(box < 4 && tinym::grouped_x_box(g.pair, box) * 128 * static_cast<int>(chunks) <= p.x_stage, "X box", box,
            p.x_stage);
-    expect(p.tn % 16 == 0 && p.tn >= 16 && p.tn <= 256 && (!g.pair || p.tn % 64 == 0) &&
+    expect(p.tn % 16 == 0 && p.tn >= 16 && p.tn <= 256 && (!g.pair || p.tn % 32 == 0) &&
                p.tn <= 128 * tinym::grouped_x_scale_blocks(g.pair),
            "tile width", p.tn);
-    const uint32_t overlap = p.tn - std::min<uint32_t>(p.tn, p.acc_cols);  // columns of both accumulators
-    expect((overlap == 0 || (g.pair && fp4 && p.acc_cols >= 2 * overlap)) && p.tmem_cols <= 512 && (p.tmem_cols & (p.tmem_cols - 1)) == 0,
+    expect(p.acc_cols >= static_cast<uint32_t>(p.tn) && p.tmem_cols <= 512 && (p.tmem_cols & (p.tmem_cols - 1)) == 0,
            "tensor memory", p.acc_cols, p.tmem_cols);
     expect((fp4 ? p.sf_col + 2 * tinym::kSfSlotCols : p.acc_cols + p.tn) <= p.tmem_cols &&
                (!fp4 || (p.sf_col >= p.acc_cols + p.tn && p.sf_col % 4 == 0)),
