@@ -58,6 +58,19 @@ constexpr int kGrpBars = 5;          // barriers beside the three per stage
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
+// n / d for 0 <= n < 2^31: multiply by ceil(2^(31 + s) / d), 2^s >= d, and shift.
+struct FastDiv {
+    uint32_t mul, shift, d;
+    __host__ static FastDiv make(uint32_t d) {
+        uint32_t s = 0;
+        while ((1ull << s) < d) ++s;
+        return {static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), 31 + s, d};
+    }
+    __host__ __device__ uint32_t div(uint32_t n) const {
+        return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
+    }
+};
+
 struct GroupedParams {
     __nv_bfloat16* y;
     const int32_t* offsets;   // null: one group over all rows
@@ -80,6 +93,7 @@ struct GroupedParams {
     uint32_t w_off, sf_off, out_off, bar_off, tab_off;  // shared-memory offsets (X ring at 0)
     int32_t wide_y;           // Y takes 16-byte stores
     uint32_t tmem_cols, acc_cols, sf_col;
+    FastDiv by_units, by_band, by_parts, by_width[kGrpBand];  // walk: units, 8 units, parts of a block, 1 .. 8
     uint32_t flags;
     uint32_t* err_host;
     uint64_t timeout_ns;
@@ -104,18 +118,15 @@ struct GroupedPiece {
 // The pieces of one CTA, in the order in which every role walks them.
 template <bool PAIR>
 struct GroupedWalk {
+    const GroupedParams& p;
     const int32_t* off;     // [experts + 1] group starts
     const int32_t* prefix;  // [experts + 1] X tiles before each group
-    int experts, n_units, units, part_units, piece_units, tn;
-    bool blocked;
     int cur, end, step;
-    int e;
+    int e, tiles, wide;  // group, its X tiles, rows of each
 
-    __host__ __device__ GroupedWalk(const GroupedParams& p, const int32_t* o, const int32_t* pre,
+    __host__ __device__ GroupedWalk(const GroupedParams& prm, const int32_t* o, const int32_t* pre,
                                     int block, int blocks)
-        : off(o), prefix(pre), experts(p.experts), n_units((p.n + 7) / 8), units(p.units),
-          part_units(p.part_units), piece_units(p.piece_units), tn(p.tn), blocked(p.blocked != 0),
-          e(-1) {
+        : p(prm), off(o), prefix(pre), e(-1), tiles(0), wide(0) {
         const int64_t total = static_cast<int64_t>(pre[p.experts]) * p.units;
         if constexpr (PAIR) {
             cur = block;
@@ -132,69 +143,72 @@ struct GroupedWalk {
 
     // First unit of part i of a matrix.
     __host__ __device__ int part_unit(int i) const {
-        const int per = (kBlockUnits + part_units - 1) / part_units;
-        return i / per * kBlockUnits + i % per * part_units;
+        const int block = static_cast<int>(p.by_parts.div(i));
+        return block * kBlockUnits + (i - block * static_cast<int>(p.by_parts.d)) * p.part_units;
     }
 
     __host__ __device__ bool next(GroupedPiece* w) {
         if constexpr (!PAIR) {
             // parts past N in a matrix's last block
-            while (part_units && cur < end && part_unit(cur % units) >= n_units) ++cur;
+            while (p.part_units && cur < end &&
+                   part_unit(cur - static_cast<int>(p.by_units.div(cur)) * p.units) * 8 >= p.n)
+                ++cur;
         }
         if (cur >= end) return false;
-        const int seg = cur / units;
+        const int seg = static_cast<int>(p.by_units.div(cur));
         if (e < 0 || seg >= prefix[e + 1]) {
-            int lo = e < 0 ? 0 : e, hi = experts - 1;  // the group whose tiles hold seg
+            int lo = e + 1, hi = p.experts - 1;  // the group whose tiles hold seg
+            for (int i = 0; i < 2 && lo < hi && prefix[lo + 1] <= seg; ++i) ++lo;  // often the next
             while (lo < hi) {
                 const int mid = (lo + hi) >> 1;
                 if (prefix[mid + 1] <= seg) lo = mid + 1;
                 else hi = mid;
             }
             e = lo;
+            // Equal tiles in whole steps of the MMA's columns: 300 rows are
+            // 160 + 140, not 256 + 44.  (tiles - 1) * wide < count, since
+            // wide <= tn.
+            constexpr int kStep = PAIR ? 32 : 16;
+            tiles = prefix[e + 1] - prefix[e];
+            wide = ((off[e + 1] - off[e] + tiles - 1) / tiles + kStep - 1) & ~(kStep - 1);
         }
-        const int tiles = prefix[e + 1] - prefix[e];
-        const int count = off[e + 1] - off[e];
         int t;
         if constexpr (PAIR) {
-            const int local = cur - prefix[e] * units;
-            const int band = local / (kGrpBand * units);
+            const int local = cur - prefix[e] * p.units;
+            const int band = static_cast<int>(p.by_band.div(local));
             const int width = least(kGrpBand, tiles - band * kGrpBand);
-            const int rem = local - band * kGrpBand * units;
-            const int wt = rem / width;
+            const int rem = local - band * kGrpBand * p.units;
+            const int wt = static_cast<int>(p.by_width[width - 1].div(rem));
             t = band * kGrpBand + rem - wt * width;
             w->w0 = wt * 2 * kTileRows;
             w->h = 2 * kTileRows;
             cur += step;
         } else {
             t = seg - prefix[e];
-            int u = cur - seg * units, take;
-            if (part_units) {
+            int u = cur - seg * p.units, take;
+            if (p.part_units) {
                 u = part_unit(u);
-                take = least(least(part_units, kBlockUnits - u % kBlockUnits), n_units - u);
+                take = least(least(p.part_units, kBlockUnits - u % kBlockUnits), (p.n + 7) / 8 - u);
                 ++cur;
             } else {
-                int left = least(end - cur, units - u);
-                if (blocked) left = least(left, kBlockUnits - u % kBlockUnits);
-                const int pieces = (left + piece_units - 1) / piece_units;
+                int left = least(end - cur, p.units - u);
+                if (p.blocked) left = least(left, kBlockUnits - u % kBlockUnits);
+                const int pieces = (left + p.piece_units - 1) / p.piece_units;
                 take = (left + pieces - 1) / pieces;
                 cur += take;
             }
             w->w0 = u * 8;
             w->h = take * 8;
         }
-        // Equal tiles in whole steps of the MMA's columns: 300 rows are 160 +
-        // 140, not 256 + 44.  (tiles - 1) * wide < count, since wide <= tn.
-        constexpr int kStep = PAIR ? 32 : 16;
-        const int wide = ((count + tiles - 1) / tiles + kStep - 1) & ~(kStep - 1);
         w->e = e;
         w->row0 = off[e] + t * wide;
-        w->rows = least(wide, count - t * wide);
+        w->rows = least(wide, off[e + 1] - w->row0);
         return true;
     }
 };
 
-// A walk that works out the next piece ahead of time (several integer
-// divisions, ~1,000 cycles), while a role has nothing urgent to do.
+// A walk that works out the next piece ahead of time (a few
+// hundred cycles of dependent steps), while a role has nothing urgent to do.
 template <bool PAIR>
 struct GroupedAhead {
     GroupedWalk<PAIR> walk;
@@ -281,6 +295,11 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.tmem_cols = 32;
         while (p.tmem_cols < 2 * p.acc_cols + (fp4 ? 2 * kSfSlotCols : 0)) p.tmem_cols *= 2;
     }
+    p.by_units = FastDiv::make(static_cast<uint32_t>(p.units));
+    p.by_band = FastDiv::make(static_cast<uint32_t>(kGrpBand * p.units));
+    p.by_parts = FastDiv::make(static_cast<uint32_t>(
+        p.part_units ? (kBlockUnits + p.part_units - 1) / p.part_units : 1));
+    for (int i = 0; i < kGrpBand; ++i) p.by_width[i] = FastDiv::make(static_cast<uint32_t>(i + 1));
     p.w_stage = p.piece_units * chunks * 1024;
     if (fp4) p.sf_stage = chunks * 2 * (1 + grouped_x_scale_blocks(g.pair)) * kScaleBlock;
     const int64_t max_items = (groups + rows / p.tn) * p.units;

@@ -27,19 +27,6 @@ namespace tinym {
 constexpr int kMxThreads = 256;
 constexpr int kMxUnroll = 4;  // 128-column groups a 16-thread team loads before it uses the first
 
-// n / d for 0 <= n < 2^31: multiply by ceil(2^(31 + s) / d), 2^s >= d, and shift.
-struct FastDiv {
-    uint32_t mul, shift, d;
-    __host__ static FastDiv make(uint32_t d) {
-        uint32_t s = 0;
-        while ((1ull << s) < d) ++s;
-        return {static_cast<uint32_t>(((1ull << (31 + s)) + d - 1) / d), 31 + s, d};
-    }
-    __device__ __forceinline__ uint32_t div(uint32_t n) const {
-        return static_cast<uint32_t>((static_cast<uint64_t>(n) * mul) >> shift);
-    }
-};
-
 struct MxParams {
     int32_t rows, k;          // rows of one matrix, columns
     int32_t row_blocks;       // ceil(rows / 128)
