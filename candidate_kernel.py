@@ -64,6 +64,7 @@ _run_alpha_tensor = None
 _run_packed = None
 _pack = None
 _run_quant_act = None
+_run_grouped = _mxfp4_quantize = _mxfp4_dequantize = _run_mxfp4 = _run_mxfp4_grouped = None
 # The alpha tensor (and its version counter) last checked finite.
 _ALPHA_TENSOR = None
 _ALPHA_VERSION = None
@@ -90,6 +91,7 @@ class PackedWeight:
 def build():
     """Load (building once if needed) the native op; returns True."""
     global _BUILT, _run_alpha_tensor, _run_packed, _pack, _run_quant_act
+    global _run_grouped, _mxfp4_quantize, _mxfp4_dequantize, _run_mxfp4, _run_mxfp4_grouped
     if _BUILT:
         return True
     with _BUILD_LOCK:
@@ -99,6 +101,11 @@ def build():
             _run_packed = torch.ops.sm120_fp8_gemm.run_packed
             _pack = torch.ops.sm120_fp8_gemm.pack_weights
             _run_quant_act = torch.ops.sm120_fp8_gemm.run_quant_act
+            _run_grouped = torch.ops.sm120_fp8_gemm.run_grouped.default
+            _mxfp4_quantize = torch.ops.sm120_fp8_gemm.mxfp4_quantize.default
+            _mxfp4_dequantize = torch.ops.sm120_fp8_gemm.mxfp4_dequantize.default
+            _run_mxfp4 = torch.ops.sm120_fp8_gemm.run_mxfp4.default
+            _run_mxfp4_grouped = torch.ops.sm120_fp8_gemm.run_mxfp4_grouped.default
             _BUILT = True
     return True
 
@@ -179,7 +186,7 @@ def fp8_gemm_grouped(a: torch.Tensor, b: torch.Tensor, alpha: torch.Tensor, offs
     if not _BUILT:
         build()
     if out is None:
-        return torch.ops.sm120_fp8_gemm.run_grouped(a, b, alpha, offsets)
+        return _run_grouped(a, b, alpha, offsets)
     torch.ops.sm120_fp8_gemm.run_grouped_out(a, b, alpha, offsets, out)
     return out
 
@@ -193,7 +200,7 @@ def mxfp4_quantize(x: torch.Tensor):
     saturated; a block that holds a NaN or an infinity becomes NaN."""
     if not _BUILT:
         build()
-    return torch.ops.sm120_fp8_gemm.mxfp4_quantize(x)
+    return _mxfp4_quantize(x)
 
 
 def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
@@ -201,7 +208,7 @@ def mxfp4_dequantize(codes: torch.Tensor, scales: torch.Tensor,
     """The values of mxfp4_quantize's result, in BF16 or FP32 (exact)."""
     if not _BUILT:
         build()
-    return torch.ops.sm120_fp8_gemm.mxfp4_dequantize(codes, scales, dtype)
+    return _mxfp4_dequantize(codes, scales, dtype)
 
 
 def mxfp4_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scales: torch.Tensor,
@@ -212,7 +219,7 @@ def mxfp4_gemm(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor, b_scale
     if not _BUILT:
         build()
     if out is None:
-        return torch.ops.sm120_fp8_gemm.run_mxfp4(a, a_scales, b, b_scales, alpha)
+        return _run_mxfp4(a, a_scales, b, b_scales, alpha)
     torch.ops.sm120_fp8_gemm.run_mxfp4_out(a, a_scales, b, b_scales, alpha, out)
     return out
 
@@ -226,7 +233,7 @@ def mxfp4_gemm_grouped(a: torch.Tensor, a_scales: torch.Tensor, b: torch.Tensor,
     if not _BUILT:
         build()
     if out is None:
-        return torch.ops.sm120_fp8_gemm.run_mxfp4_grouped(a, a_scales, b, b_scales, offsets, alpha)
+        return _run_mxfp4_grouped(a, a_scales, b, b_scales, offsets, alpha)
     torch.ops.sm120_fp8_gemm.run_mxfp4_grouped_out(a, a_scales, b, b_scales, offsets, alpha, out)
     return out
 

@@ -93,7 +93,7 @@ struct GroupedParams {
     uint32_t w_off, sf_off, out_off, bar_off, tab_off;  // shared-memory offsets (X ring at 0)
     int32_t wide_y;           // Y takes 16-byte stores
     uint32_t tmem_cols, acc_cols, sf_col;
-    FastDiv by_units, by_band, by_parts, by_width[kGrpBand];  // walk: units, 8 units, parts of a block, 1 .. 8
+    FastDiv by_grid, by_units, by_band, by_parts, by_width[kGrpBand];  // walk: CTAs, units, 8 units, parts of a block, 1 .. 8
     uint32_t flags;
     uint32_t* err_host;
     uint64_t timeout_ns;
@@ -127,14 +127,17 @@ struct GroupedWalk {
     __host__ __device__ GroupedWalk(const GroupedParams& prm, const int32_t* o, const int32_t* pre,
                                     int block, int blocks)
         : p(prm), off(o), prefix(pre), e(-1), tiles(0), wide(0) {
-        const int64_t total = static_cast<int64_t>(pre[p.experts]) * p.units;
+        const int total = pre[p.experts] * p.units;  // below 2^31 (grouped_plan)
         if constexpr (PAIR) {
             cur = block;
-            end = static_cast<int>(total);
+            end = total;
             step = blocks;
         } else {
-            cur = static_cast<int>(total * block / blocks);
-            end = static_cast<int>(total * (block + 1) / blocks);
+            // shares of total / blocks units, the first ones one more
+            const int share = static_cast<int>(p.by_grid.div(total));
+            const int more = total - share * blocks;
+            cur = block * share + least(block, more);
+            end = cur + share + (block < more ? 1 : 0);
             step = 0;
         }
     }
@@ -170,7 +173,9 @@ struct GroupedWalk {
             // wide <= tn.
             constexpr int kStep = PAIR ? 32 : 16;
             tiles = prefix[e + 1] - prefix[e];
-            wide = ((off[e + 1] - off[e] + tiles - 1) / tiles + kStep - 1) & ~(kStep - 1);
+            int count = off[e + 1] - off[e];
+            if (tiles > 1) count = (count + tiles - 1) / tiles;
+            wide = (count + kStep - 1) & ~(kStep - 1);
         }
         int t;
         if constexpr (PAIR) {
@@ -193,8 +198,8 @@ struct GroupedWalk {
             } else {
                 int left = least(end - cur, p.units - u);
                 if (p.blocked) left = least(left, kBlockUnits - u % kBlockUnits);
-                const int pieces = (left + p.piece_units - 1) / p.piece_units;
-                take = (left + pieces - 1) / pieces;
+                take = left <= p.piece_units ? left
+                       : left < 2 * p.piece_units ? (left + 1) / 2 : p.piece_units;
                 cur += take;
             }
             w->w0 = u * 8;
@@ -307,6 +312,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     g.grid = static_cast<int>(g.pair ? 2 * std::min<int64_t>(sm_count / 2, max_items)
                                      : std::min<int64_t>(sm_count, max_items));
 
+    p.by_grid = FastDiv::make(static_cast<uint32_t>(g.grid));
     const uint32_t tables = 8u * static_cast<uint32_t>(experts + 1);
     auto bytes_for = [&](int stages) -> uint32_t {
         p.stages = stages;
@@ -609,6 +615,10 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const int nkb = (k_chunks + kChunks - 1) / kChunks;
     auto at_rank = [&](uint32_t addr, int r) { return PAIR ? dsmem_map(addr, r) : addr; };
 
+    if (threadIdx.x == 96) {  // the maps that the first stage is likely to use
+        tma_prefetch_desc(&maps.w[p.piece_units - 1]);
+        tma_prefetch_desc(&maps.x[0]);
+    }
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
             // full: the producer's expect_tx (and the bytes), the scales, and
@@ -648,9 +658,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     // X rows that this CTA loads, and the box that holds them.
     auto x_cols = [&]() { return PAIR ? ((w.rows + 31) & ~31) / 2 : w.rows; };
     auto x_box = [&](int cols) {
-        int i = 0;
-        while (grouped_x_box(PAIR, i) < cols) ++i;
-        return i;
+        return 32 - __clz((cols - 1) / grouped_x_box(PAIR, 0));  // log2 of the boxes of 8 or 16, rounded up
     };
 
     if (warp == 0) {
@@ -670,7 +678,9 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             const CUtensorMap* mw = &maps.w[w_rows / 8 - 1];
             const CUtensorMap* mx = &maps.x[xi];
             for (int i = 0; i < nkb; ++i) {
-                if (!(ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait))) break;
+                if (issued >= stages &&
+                    !(ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait)))
+                    break;
                 const uint32_t wd = w_ring + s * p.w_stage, xd = x_ring + s * p.x_stage;
                 const uint32_t bar = full_bar(s);
                 const int c0 = i * kChunks;
@@ -987,13 +997,16 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         int piece = 0;
         while (walk.next(&w)) {
             const int b = piece & 1;
+            // ahead of the wait, so that its latency is hidden
+            float alpha = 1.0f;
+            if (p.alpha)
+                asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(alpha) : "l"(p.alpha + w.e * p.alpha_stride) : "memory");
             walk.ahead();
             if (!warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait)) break;
             // The MMAs' commit reaches CTA 0 alone: pass it on.
             if (PAIR && rank == 0 && warp == 4 && lane == 0)
                 mbar_arrive_remote(at_rank(acc_full(b), 1));
             tc_fence_after_sync();
-            const float alpha = p.alpha ? __ldg(p.alpha + w.e * p.alpha_stride) : 1.0f;
             const uint32_t taddr = tmem + b * p.acc_cols + (static_cast<uint32_t>(q * 32) << 16);
             __nv_bfloat16* row0 = p.y + static_cast<int64_t>(w.row0) * p.ldy;
             if constexpr (PAIR) {
