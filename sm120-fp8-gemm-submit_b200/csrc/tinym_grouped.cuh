@@ -22,7 +22,8 @@
 //    walked in pieces of at most 128 rows with the whole of K.  The shares
 //    differ by at most one unit, so every SM streams the same number of bytes
 //    whatever the groups are, with no split of K, no workspace and one fixed
-//    order of every sum.  A stage is 512 bytes of K.
+//    order of every sum.  A stage is 512 bytes of K
+//    (256 bytes took 10 % longer on one-token calls, 4 % on decode batches).
 //  * Pair pieces (PAIR = true), for many rows per group, where the time is the
 //    tensor core's: two CTAs (cta_group::2) compute 256 W rows x up to 256 X
 //    rows, 128 bytes of K a stage.  Each loads its 128 W rows and half of the
@@ -54,6 +55,7 @@ constexpr int kGrpThreads = 256;     // warp 0 TMA, 1 MMA, 2-3 scales, 4-7 epilo
 constexpr int kGrpMaxExperts = 1024;
 constexpr int kGrpBand = 8;          // row tiles walked together for each W tile (L2 reuse)
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
+constexpr int kStreamChunks = 4;     // 128-byte chunks of K in a stream stage
 constexpr int kGrpBars = 5;          // barriers beside the three per stage
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
@@ -259,7 +261,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     p.n = static_cast<int32_t>(n);
     p.k_bytes = static_cast<int32_t>(k_bytes);
     const int64_t k_chunks = (k_bytes + kBlockK - 1) / kBlockK;
-    const int chunks = g.pair ? 1 : 4;  // of a stage
+    const int chunks = g.pair ? 1 : kStreamChunks;  // of a stage
     const int64_t nkb = (k_chunks + chunks - 1) / chunks;
     // Bytes in front of the W ring that an MMA may read: a piece that starts
     // inside a scale block stands that many rows into the MMA's rows.
@@ -320,7 +322,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.w_off = p.sf_off + static_cast<uint32_t>(stages * p.sf_stage);
         p.w_off = (std::max(p.w_off, front) + 1023u) & ~1023u;
         p.out_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
-        p.bar_off = p.out_off + (g.pair ? 4 * kOutBytes : 0);
+        p.bar_off = p.out_off + 4 * kOutBytes;
         p.tab_off = p.bar_off + 8u * (3 * stages + kGrpBars) + 8u;
         // The MMA's 128 W rows of the last chunk end inside the allocation.
         const uint32_t read_end = p.w_off + static_cast<uint32_t>(stages * p.w_stage) + kTileRows * kBlockK;
@@ -497,25 +499,14 @@ __device__ __forceinline__ void cp_async_wait_all() {
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-__device__ __forceinline__ void tmem_ld_x16_nowait(uint32_t taddr, uint32_t* r) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-        : "r"(taddr));
-}
-// 16 lanes x 32 columns as the fragments of 8 x 8 matrices: for columns 8 j ..
+// 16 lanes x 16 columns as the fragments of 8 x 8 matrices: for columns 8 j ..
 // r[4 j], r[4 j + 1] are lane t / 4, columns 2 (t % 4) and + 1, the next two
 // lane t / 4 + 8.
 __device__ __forceinline__ void tmem_ld_frag(uint32_t taddr, uint32_t* r) {
     asm volatile(
-        "tcgen05.ld.sync.aligned.16x256b.x4.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        "tcgen05.ld.sync.aligned.16x256b.x2.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-          "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+          "=r"(r[7])
         : "r"(taddr));
 }
 // Four 8 x 8 matrices of 16-bit values, transposed, to the row addresses that
@@ -582,7 +573,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     tinym_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) {
     using Ops = Tc<PAIR ? 2 : 1>;
     constexpr int kCtas = PAIR ? 2 : 1;
-    constexpr int kChunks = PAIR ? 1 : 4;  // 128-byte chunks of K per stage
+    constexpr int kChunks = PAIR ? 1 : kStreamChunks;  // 128-byte chunks of K per stage
     constexpr int kMmaK = 32;              // bytes of K per MMA (32 E4M3 or 64 E2M1 elements)
     constexpr int kSfPerChunk = 2;         // MXFP4: scale blocks (128 elements) per chunk
     constexpr int kXsBlocks = grouped_x_scale_blocks(PAIR);
@@ -951,6 +942,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                             }
                             cp_async_arrive(sf_bar(s));
                         } else {
+#pragma unroll
                             for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
                                 const uint32_t mask = block_mask(b0 + q);
                                 const int64_t at = static_cast<int64_t>(min(b0 + q, blocks - 1)) * kScaleBlock;
@@ -1009,79 +1001,65 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             tc_fence_after_sync();
             const uint32_t taddr = tmem + b * p.acc_cols + (static_cast<uint32_t>(q * 32) << 16);
             __nv_bfloat16* row0 = p.y + static_cast<int64_t>(w.row0) * p.ldy;
-            if constexpr (PAIR) {
-                const int n0 = w.w0 + rank * kTileRows + q * 32;  // this warp's first W row
-                // 32 X rows at a time through shared memory, [X row][32 W rows]
-                // of BF16 with the 16-byte chunks of a row exchanged so that
-                // neither side has bank conflicts.
-                uint8_t* buf = smem + p.out_off + q * kOutBytes;
-                for (int c = 0; c < w.rows; c += 32) {
-                    uint32_t v[2][16];
-                    tmem_ld_frag(taddr + c, v[0]);
-                    tmem_ld_frag(taddr + (16u << 16) + c, v[1]);
-                    tmem_ld_wait();
-                    if (c + 32 >= w.rows) {  // everything is read: the accumulator is free
-                        tc_fence_before_sync();
-                        __syncwarp();
-                        if (lane == 0) {
-                            if (rank) mbar_arrive_remote(at_rank(acc_empty(b), 0));
-                            else mbar_arrive(acc_empty(b));
-                        }
-                    }
-                    if (n0 >= p.n) continue;
+            // W rows of this warp's TMEM lanes, and those of them in the piece.
+            const int n0 = w.w0 + rank * kTileRows - first_row() + q * 32;
+            const int n_lo = PAIR ? n0 : w.w0;
+            const int n_hi = min(p.n, PAIR ? n0 + 32 : w.w0 + w.h);
+            // kCols X rows at a time through shared memory, [X row][32 W rows]
+            // of BF16 with the 16-byte chunks of a row exchanged so that
+            // neither side has bank conflicts, to 16-byte stores.
+            constexpr int kCols = PAIR ? 32 : 16;
+            uint8_t* buf = smem + p.out_off + q * kOutBytes;
+            for (int c = 0; c < w.rows; c += kCols) {
+                uint32_t v[2][kCols / 2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-#pragma unroll
-                        for (int g = 0; g < 4; g += 2) {
-                            const int r = 8 * (g + (lane >> 4)) + (lane & 7);
-                            const int ch = 2 * h + ((lane >> 3) & 1);
-                            const uint32_t* f = v[h] + 4 * g;
-                            stmatrix_x4_trans(smem_u32(buf) + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16),
-                                              pack_bf16(f[0], f[1], alpha), pack_bf16(f[2], f[3], alpha),
-                                              pack_bf16(f[4], f[5], alpha), pack_bf16(f[6], f[7], alpha));
-                        }
-                    __syncwarp();
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) {
-                        const int r = 8 * k + (lane >> 2), ch = lane & 3;
-                        const int n = n0 + ch * 8;
-                        const uint4 o = *reinterpret_cast<const uint4*>(
-                            buf + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16));
-                        if (c + r < w.rows && n < p.n) {
-                            __nv_bfloat16* dst = row0 + (c + r) * p.ldy + n;
-                            if (p.wide_y && n + 8 <= p.n) {
-                                *reinterpret_cast<uint4*>(dst) = o;
-                            } else {
-                                const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
-#pragma unroll
-                                for (int i = 0; i < 8; ++i)
-                                    if (n + i < p.n)
-                                        reinterpret_cast<uint16_t*>(dst)[i] =
-                                            static_cast<uint16_t>(ow[i / 2] >> (16 * (i & 1)));
-                            }
-                        }
-                    }
-                    __syncwarp();
+                for (int g = 0; g < kCols; g += 16) {
+                    tmem_ld_frag(taddr + c + g, v[0] + g / 2);
+                    tmem_ld_frag(taddr + (16u << 16) + c + g, v[1] + g / 2);
                 }
-            } else {
-                const int r = q * 32 + lane - first_row();  // W row of the piece
-                const int n = w.w0 + r;
-                const bool mine = r >= 0 && r < w.h && n < p.n;
-                for (int c = 0; c < w.rows; c += 16) {
-                    uint32_t v[16];
-                    tmem_ld_x16_nowait(taddr + c, v);
-                    tmem_ld_wait();
-                    if (mine) {
-#pragma unroll
-                        for (int h = 0; h < 16; ++h)
-                            if (c + h < w.rows)
-                                row0[(c + h) * p.ldy + n] =
-                                    __float2bfloat16_rn(__uint_as_float(v[h]) * alpha);
+                tmem_ld_wait();
+                if (c + kCols >= w.rows) {  // everything is read: the accumulator is free
+                    tc_fence_before_sync();
+                    __syncwarp();
+                    if (lane == 0) {
+                        if (rank) mbar_arrive_remote(at_rank(acc_empty(b), 0));
+                        else mbar_arrive(acc_empty(b));
                     }
                 }
-                tc_fence_before_sync();
+                if (n0 >= n_hi || n0 + 32 <= n_lo) continue;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int g = 0; g < kCols / 8; g += 2) {
+                        const int r = 8 * (g + (lane >> 4)) + (lane & 7);
+                        const int ch = 2 * h + ((lane >> 3) & 1);
+                        const uint32_t* f = v[h] + 4 * g;
+                        stmatrix_x4_trans(smem_u32(buf) + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16),
+                                          pack_bf16(f[0], f[1], alpha), pack_bf16(f[2], f[3], alpha),
+                                          pack_bf16(f[4], f[5], alpha), pack_bf16(f[6], f[7], alpha));
+                    }
                 __syncwarp();
-                if (lane == 0) mbar_arrive(acc_empty(b));
+#pragma unroll
+                for (int k = 0; k < kCols / 8; ++k) {
+                    const int r = 8 * k + (lane >> 2), ch = lane & 3;
+                    const int n = n0 + ch * 8;
+                    const uint4 o = *reinterpret_cast<const uint4*>(
+                        buf + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16));
+                    if (c + r < w.rows && n >= n_lo && n < n_hi) {
+                        __nv_bfloat16* dst = row0 + (c + r) * p.ldy + n;
+                        if (p.wide_y && n + 8 <= n_hi) {
+                            *reinterpret_cast<uint4*>(dst) = o;
+                        } else {
+                            const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (n + i < n_hi)
+                                    reinterpret_cast<uint16_t*>(dst)[i] =
+                                        static_cast<uint16_t>(ow[i / 2] >> (16 * (i & 1)));
+                        }
+                    }
+                }
+                __syncwarp();
             }
             ++piece;
         }

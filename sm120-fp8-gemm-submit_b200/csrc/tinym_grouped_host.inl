@@ -121,7 +121,7 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
                     (long long)rows, (long long)experts, (long long)n);
     GroupedParams& p = g.prm;
     // A map per box height that the pieces can have.
-    const int chunks = !g.pair && p.chunked ? 4 : 1;
+    const int chunks = !g.pair && p.chunked ? tinym::kStreamChunks : 1;
     tinym::GroupedMaps maps;
     for (int i = g.pair ? tinym::kBlockUnits - 1 : 0; i < p.piece_units; ++i)
         if ((st = encode_stack(w, experts, n, k_bytes, 8 * (i + 1), chunks, &maps.w[i])) != TINYM_OK)
@@ -186,7 +186,8 @@ int check_scales(const void* xs, const void* ws) {
     return TINYM_OK;
 }
 
-int mx_params(int64_t batch, int64_t rows, int64_t k, MxParams* p) {
+// run: columns that one warp takes (256 * kMxSteps).
+int mx_params(int64_t batch, int64_t rows, int64_t k, int64_t run, MxParams* p) {
     if (batch < 1 || rows < 1 || k < 1)
         return fail(TINYM_ERR_INVALID_ARGUMENT, "batch, rows and K must be positive (got %lld, %lld, %lld)",
                     (long long)batch, (long long)rows, (long long)k);
@@ -201,8 +202,10 @@ int mx_params(int64_t batch, int64_t rows, int64_t k, MxParams* p) {
     p->rows = static_cast<int32_t>(rows);
     p->k = static_cast<int32_t>(k);
     p->row_blocks = static_cast<int32_t>(rb);
-    p->groups = static_cast<uint32_t>(batch * rows * kc);
+    const int64_t per_row = (k + run - 1) / run;
+    p->runs = static_cast<uint32_t>(batch * rows * per_row);
     p->pad_words = static_cast<uint32_t>(batch * pad * kc);
+    p->per_row = tinym::FastDiv::make(static_cast<uint32_t>(per_row));
     p->kc = tinym::FastDiv::make(static_cast<uint32_t>(kc));
     p->per_matrix = tinym::FastDiv::make(static_cast<uint32_t>(rows));
     p->pad_per_matrix = tinym::FastDiv::make(static_cast<uint32_t>(std::max<int64_t>(1, pad)));
@@ -216,7 +219,8 @@ int mx_launch(bool quantize, const void* wide, int32_t dtype, const void* codes,
     if (dtype != TINYM_ACT_BF16 && dtype != TINYM_ACT_F32)
         return fail(TINYM_ERR_INVALID_ARGUMENT, "dtype %d is not TINYM_ACT_BF16 / TINYM_ACT_F32", dtype);
     MxParams p{};
-    int st = mx_params(batch, rows, k, &p);
+    const int64_t run = 256 * (dtype == TINYM_ACT_BF16 ? tinym::kMxSteps<__nv_bfloat16> : tinym::kMxSteps<float>);
+    int st = mx_params(batch, rows, k, run, &p);
     if (st != TINYM_OK) return st;
     if ((reinterpret_cast<uintptr_t>(wide) & 15u) || (reinterpret_cast<uintptr_t>(codes) & 15u) ||
         (reinterpret_cast<uintptr_t>(scales) & 15u))
@@ -226,9 +230,9 @@ int mx_launch(bool quantize, const void* wide, int32_t dtype, const void* codes,
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
     DeviceInfo* di = nullptr;
     if ((st = device_info(dev, &di)) != TINYM_OK) return st;
-    const int64_t teams_per_cta = tinym::kMxThreads / 16;
+    constexpr int kWarps = tinym::kMxThreads / 32;
     const int64_t want = std::max<int64_t>(
-        (p.groups + teams_per_cta - 1) / teams_per_cta,
+        (p.runs + kWarps - 1) / kWarps,
         quantize ? (p.pad_words + tinym::kMxThreads - 1) / tinym::kMxThreads : 1);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(want, int64_t(di->sm_count) * 8));
     auto s = static_cast<cudaStream_t>(stream);
@@ -298,7 +302,7 @@ int tinym_mxfp4_scale_bytes(int64_t batch, int64_t rows, int64_t k, int64_t* byt
     t_last_error[0] = '\0';
     if (!bytes) return fail(TINYM_ERR_INVALID_ARGUMENT, "bytes is NULL");
     MxParams p{};
-    const int st = mx_params(batch, rows, k, &p);
+    const int st = mx_params(batch, rows, k, 128, &p);
     if (st != TINYM_OK) return st;
     *bytes = batch * p.row_blocks * p.kc.d * tinym::kScaleBlock;
     return TINYM_OK;
