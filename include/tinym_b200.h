@@ -317,8 +317,8 @@ TINYM_API int tinym_ipc_close(void* base);
  * alpha_dev: alpha_count = 1 value for all experts, or `experts` values; NULL
  * means 1.  It is used as it is (a non-finite alpha gives non-finite rows).
  * Any number of rows >= 1 and any N; K % 16 == 0; up to 1024 experts.  Sums
- * are FP32 over the whole of K in one fixed order: a row's result depends
- * neither on the run nor on the split of the work over SMs.
+ * are FP32 in an order that the shapes (rows, experts, N, K) fix: a row's
+ * result depends neither on the run nor on the groups of the other rows.
  */
 #define TINYM_FLAG_ZERO_REST 2u
 TINYM_API int tinym_fp8_gemm_grouped(const void* x, const void* w, void* y, int64_t ldy,

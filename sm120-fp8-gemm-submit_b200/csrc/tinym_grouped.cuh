@@ -16,7 +16,7 @@
 // groups' row tiles in shared memory and every role of the CTA walks the same
 // list of pieces (group, row tile, W rows).
 //
-//  * Stream pieces (PAIR = false), for few rows per group, where the time is
+//  * Stream pieces, for few rows per group, where the time is
 //    W's bytes: the W rows of all non-empty groups are laid end to end in
 //    units of 8 rows and each CTA takes an equal, contiguous share of them,
 //    walked in pieces of at most 128 rows with the whole of K.  The shares
@@ -24,7 +24,14 @@
 //    whatever the groups are, with no split of K, no workspace and one fixed
 //    order of every sum.  A stage is 512 bytes of K
 //    (256 bytes took 10 % longer on one-token calls, 4 % on decode batches).
-//  * Pair pieces (PAIR = true), for many rows per group, where the time is the
+//  * Folded stream pieces (FOLD), for so little work that a CTA's share is at
+//    most 64 W rows and a tile at most 16 X rows.  An MMA costs ~45 cycles to
+//    issue whether 30 or 128 of its rows are used, and a share takes K / 32
+//    bytes of them.  So K is cut into S segments that stand side by side in
+//    one MMA: A row a h + r is W row r in segment a, B column b x + t is X row
+//    t in segment b, the S diagonal blocks of the product are the segments'
+//    sums, and the epilogue adds them in order: a S-th of the instructions.
+//  * Pair pieces, for many rows per group, where the time is the
 //    tensor core's: two CTAs (cta_group::2) compute 256 W rows x up to 256 X
 //    rows, 128 bytes of K a stage.  Each loads its 128 W rows and half of the
 //    X rows, so a CTA moves 256 rows of K for 128 x 256 sums where one CTA
@@ -57,6 +64,7 @@ constexpr int kGrpBand = 8;          // row tiles walked together for each W til
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
 constexpr int kStreamChunks = 4;     // 128-byte chunks of K in a stream stage
 constexpr int kGrpBars = 5;          // barriers beside the three per stage
+constexpr int kFoldOutBytes = kTileRows * 17 * 4;  // folded: FP32 sums of 128 MMA rows x 16 X rows
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
@@ -90,7 +98,8 @@ struct GroupedParams {
     int32_t piece_units;      // stream: units per piece, at most
     int32_t blocked;          // stream: pieces stay inside 128-row blocks (MXFP4)
     int32_t stages;
-    int32_t chunked;          // stream: one box per unit covers the whole stage
+    int32_t chunked;          // stream: one box covers a whole stage (K a multiple of 128 bytes)
+    int32_t fold, fold_x;     // folded: segments of K, X rows of a segment's columns (8 or 16)
     int32_t w_stage, x_stage, sf_stage;  // bytes
     uint32_t w_off, sf_off, out_off, bar_off, tab_off;  // shared-memory offsets (X ring at 0)
     int32_t wide_y;           // Y takes 16-byte stores
@@ -104,6 +113,9 @@ struct GroupedParams {
 struct GroupedMaps {
     CUtensorMap w[kTileRows / 8];
     CUtensorMap x[4];
+    // stream, K no multiple of 128 bytes: boxes of one chunk for the last stage
+    CUtensorMap w_tail[kTileRows / 8];
+    CUtensorMap x_tail[4];
 };
 __host__ __device__ constexpr int grouped_x_box(bool pair, int i) { return (pair ? 16 : 8) << i; }
 constexpr uint32_t kGrpZeroRest = 1u;  // rows of no group are written as zeros
@@ -238,8 +250,10 @@ struct GroupedAhead {
 };
 
 // How a call is cut.
+enum GroupedMode { kStream, kFold, kPair };
 struct GroupedPlan {
-    bool pair;
+    GroupedMode mode;
+    bool pair;  // mode == kPair
     int grid;
     uint32_t smem;
     GroupedParams prm;  // the shape and layout fields
@@ -256,13 +270,13 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     const int64_t groups = std::min(experts, rows);
     const int64_t avg = (rows + groups - 1) / groups;
     g.pair = avg > 64;
+    g.mode = g.pair ? kPair : kStream;
     p.rows = static_cast<int32_t>(rows);
     p.experts = static_cast<int32_t>(experts);
     p.n = static_cast<int32_t>(n);
     p.k_bytes = static_cast<int32_t>(k_bytes);
     const int64_t k_chunks = (k_bytes + kBlockK - 1) / kBlockK;
     const int chunks = g.pair ? 1 : kStreamChunks;  // of a stage
-    const int64_t nkb = (k_chunks + chunks - 1) / chunks;
     // Bytes in front of the W ring that an MMA may read: a piece that starts
     // inside a scale block stands that many rows into the MMA's rows.
     const uint32_t front = fp4 && !g.pair ? kTileRows * kBlockK : 0;
@@ -278,12 +292,25 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.sf_col = 448;
         p.tmem_cols = 512;
     } else {
-        p.tn = static_cast<int32_t>(std::min<int64_t>(64, (3 * avg + 15) / 16 * 16));
+        // Room for a group of three times the average; a single group is known.
+        p.tn = static_cast<int32_t>(std::min<int64_t>(64, ((experts == 1 ? 1 : 3) * avg + 15) / 16 * 16));
         const int64_t n_units = (n + 7) / 8, blocks = (n_units + kBlockUnits - 1) / kBlockUnits;
         p.units = static_cast<int32_t>(n_units);
         p.blocked = fp4 ? 1 : 0;
         p.chunked = k_bytes % kBlockK == 0;
-        if (fp4 && groups * blocks < sm_count) {
+        const int64_t share = (groups * n_units + sm_count - 1) / sm_count;
+        if (p.tn == 16 && p.chunked && share <= kBlockUnits / 2) {
+            // The most segments that divide K's chunks, fit 128 MMA rows and
+            // keep the MMA at 64 columns (where its time starts to grow).
+            p.fold_x = rows <= 8 ? 8 : 16;
+            for (int s = 2; s * share <= kBlockUnits && s * p.fold_x <= 64; ++s)
+                if (k_chunks % s == 0) p.fold = s;
+        }
+        if (p.fold) {
+            g.mode = kFold;
+            p.blocked = 0;
+            p.piece_units = static_cast<int32_t>(share);
+        } else if (fp4 && groups * blocks < sm_count) {
             // Less than a block per SM: equal parts of a block, one piece each
             // (a share that crosses a block would take two passes over K).
             const int per = static_cast<int>(std::min<int64_t>(kBlockUnits, sm_count / (groups * blocks)));
@@ -291,13 +318,16 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
             p.units = static_cast<int32_t>(blocks * ((kBlockUnits + p.part_units - 1) / p.part_units));
             p.piece_units = p.part_units;
         } else {
-            const int64_t share = (groups * n_units + sm_count - 1) / sm_count;
             p.piece_units = static_cast<int32_t>(fp4 ? kBlockUnits : std::min<int64_t>(kBlockUnits, share));
         }
         int x_rows = 8;
         while (x_rows < p.tn) x_rows *= 2;
-        p.x_stage = x_rows * chunks * kBlockK;
         p.acc_cols = static_cast<uint32_t>(p.tn);
+        if (p.fold) {
+            x_rows = p.fold * p.fold_x;
+            p.acc_cols = static_cast<uint32_t>((x_rows + 15) / 16 * 16);
+        }
+        p.x_stage = x_rows * chunks * kBlockK;
         p.sf_col = 2 * p.acc_cols;
         p.tmem_cols = 32;
         while (p.tmem_cols < 2 * p.acc_cols + (fp4 ? 2 * kSfSlotCols : 0)) p.tmem_cols *= 2;
@@ -307,7 +337,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     p.by_parts = FastDiv::make(static_cast<uint32_t>(
         p.part_units ? (kBlockUnits + p.part_units - 1) / p.part_units : 1));
     for (int i = 0; i < kGrpBand; ++i) p.by_width[i] = FastDiv::make(static_cast<uint32_t>(i + 1));
-    p.w_stage = p.piece_units * chunks * 1024;
+    p.w_stage = std::max(1, p.fold) * p.piece_units * chunks * 1024;
     if (fp4) p.sf_stage = chunks * 2 * (1 + grouped_x_scale_blocks(g.pair)) * kScaleBlock;
     const int64_t max_items = (groups + rows / p.tn) * p.units;
     if (max_items > (int64_t(1) << 31) - (int64_t(1) << 20)) return "too many tiles";
@@ -322,12 +352,14 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.w_off = p.sf_off + static_cast<uint32_t>(stages * p.sf_stage);
         p.w_off = (std::max(p.w_off, front) + 1023u) & ~1023u;
         p.out_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
-        p.bar_off = p.out_off + 4 * kOutBytes;
+        p.bar_off = p.out_off + (p.fold ? kFoldOutBytes : 4 * kOutBytes);
         p.tab_off = p.bar_off + 8u * (3 * stages + kGrpBars) + 8u;
         // The MMA's 128 W rows of the last chunk end inside the allocation.
         const uint32_t read_end = p.w_off + static_cast<uint32_t>(stages * p.w_stage) + kTileRows * kBlockK;
         return std::max(p.tab_off + tables, g.pair ? 0u : read_end) + 1024u;
     };
+    const int64_t seg_chunks = k_chunks / std::max(1, p.fold);
+    const int64_t nkb = (seg_chunks + chunks - 1) / chunks;
     int stages = static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(12, 2 * nkb)));
     while (stages >= 2 && bytes_for(stages) > smem_limit) --stages;
     if (stages < 2) return "no two stages fit";
@@ -465,6 +497,31 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const W
     return true;
 }
 
+__device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                            int32_t c0, int32_t c1, int32_t c2, int32_t c3, int32_t c4,
+                                            uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint"
+        " [%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4),
+        "l"(policy)
+        : "memory");
+}
+
+// Whether `ok` holds in all 128 epilogue threads (named barrier 1).
+__device__ __forceinline__ bool epilogue_all(bool ok) {
+    uint32_t all;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.u32 p, %1, 0;\n\t"
+        "barrier.cta.red.and.pred q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}\n"
+        : "=r"(all)
+        : "r"(ok ? 1u : 0u)
+        : "memory");
+    return all != 0;
+}
+
 __device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
@@ -568,9 +625,10 @@ __device__ __forceinline__ void grouped_tables(const GroupedParams& p, int32_t* 
     }
 }
 
-template <bool FP4, bool PAIR>
+template <bool FP4, GroupedMode MODE>
 __global__ void __launch_bounds__(kGrpThreads, 1)
     tinym_grouped_kernel(const __grid_constant__ GroupedMaps maps, const GroupedParams p) {
+    constexpr bool PAIR = MODE == kPair, FOLD = MODE == kFold;
     using Ops = Tc<PAIR ? 2 : 1>;
     constexpr int kCtas = PAIR ? 2 : 1;
     constexpr int kChunks = PAIR ? 1 : kStreamChunks;  // 128-byte chunks of K per stage
@@ -602,7 +660,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const int lane = threadIdx.x & 31;
     const int rank = PAIR ? static_cast<int>(cluster_ctarank()) : 0;  // 0 issues the pair's MMAs
     const WaitGuard guard{abort_flag, &g_err_word, p.timeout_ns, p.err_host};
-    const int k_chunks = (p.k_bytes + kBlockK - 1) / kBlockK;
+    // of K, or of a segment of it
+    const int k_chunks = FOLD ? p.k_bytes / kBlockK / p.fold : (p.k_bytes + kBlockK - 1) / kBlockK;
     const int nkb = (k_chunks + kChunks - 1) / kChunks;
     auto at_rank = [&](uint32_t addr, int r) { return PAIR ? dsmem_map(addr, r) : addr; };
 
@@ -645,12 +704,13 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     GroupedAhead<PAIR> walk(p, off, prefix, blockIdx.x / kCtas, gridDim.x / kCtas);
     GroupedPiece w;
     // MMA row of a stream piece's first W row (0 unless scales are blocked).
-    auto first_row = [&]() { return !PAIR && FP4 ? w.w0 % kTileRows : 0; };
+    auto first_row = [&]() { return MODE == kStream && FP4 ? w.w0 % kTileRows : 0; };
     // X rows that this CTA loads, and the box that holds them.
-    auto x_cols = [&]() { return PAIR ? ((w.rows + 31) & ~31) / 2 : w.rows; };
+    auto x_cols = [&]() { return PAIR ? ((w.rows + 31) & ~31) / 2 : FOLD ? p.fold_x : w.rows; };
     auto x_box = [&](int cols) {
         return 32 - __clz((cols - 1) / grouped_x_box(PAIR, 0));  // log2 of the boxes of 8 or 16, rounded up
     };
+    const int segs = FOLD ? p.fold : 1;
 
     if (warp == 0) {
         // ---------------- TMA producer (the whole warp walks, one lane issues)
@@ -683,18 +743,24 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                         mbar_expect_tx(bar, (kTileRows + x_rows) * kBlockK);
                         tma_load_3d(wd, mw, bar, c0 * kBlockK, w_row, w.e, pol_w);
                         tma_load_3d(xd, mx, bar, c0 * kBlockK, x_row, 0, pol_x);
-                    } else if (p.chunked) {
+                    } else if constexpr (FOLD) {
+                        mbar_expect_tx(bar, segs * (w_rows + x_rows) * kChunks * kBlockK);
+                        tma_load_5d(wd, mw, bar, 0, w_row, 0, c0, w.e, pol_w);
+                        tma_load_4d(xd, mx, bar, 0, x_row, 0, c0, pol_x);
+                    } else if (p.chunked || i < nkb - 1) {
                         mbar_expect_tx(bar, (w_rows + x_rows) * kChunks * kBlockK);
                         tma_load_4d(wd, mw, bar, 0, w_row, c0, w.e, pol_w);
                         tma_load_4d(xd, mx, bar, 0, x_row, c0, 0, pol_x);
                     } else {
+                        // K ends inside a chunk: the last stage's boxes are chunks
                         const int nc = min(kChunks, k_chunks - c0);
+                        const CUtensorMap* tw = &maps.w_tail[w_rows / 8 - 1];
                         mbar_expect_tx(bar, (w_rows + x_rows) * nc * kBlockK);
                         for (int c = 0; c < nc; ++c) {
-                            tma_load_3d(wd + c * w_rows * kBlockK, mw, bar, (c0 + c) * kBlockK, w_row,
+                            tma_load_3d(wd + c * w_rows * kBlockK, tw, bar, (c0 + c) * kBlockK, w_row,
                                         w.e, pol_w);
-                            tma_load_3d(xd + c * x_rows * kBlockK, mx, bar, (c0 + c) * kBlockK, x_row,
-                                        0, pol_x);
+                            tma_load_3d(xd + c * x_rows * kBlockK, &maps.x_tail[xi], bar, (c0 + c) * kBlockK,
+                                        x_row, 0, pol_x);
                         }
                     }
                 }
@@ -725,7 +791,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             bool ok = true;
             while (ok && walk.next(&w)) {
                 const int b = piece & 1;
-                const uint32_t mma_n = PAIR ? (w.rows + 31) & ~31 : (w.rows + 15) & ~15;
+                const uint32_t mma_n = PAIR ? (w.rows + 31) & ~31
+                                            : ((FOLD ? segs * p.fold_x : w.rows) + 15) & ~15;
                 const uint32_t idesc = FP4 ? idesc_mxf4(kCtas * 128, mma_n)
                                            : idesc_e4m3_f32(kCtas * 128, mma_n);
                 const uint32_t acc = tmem_u + b * p.acc_cols;
@@ -735,8 +802,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                 tc_fence_after_sync();
                 // Bytes from chunk to chunk of a stage, and of the rows that
                 // stand in front of a blocked piece's first one.
-                const int w_chunk = (PAIR ? kTileRows : w.h) * kBlockK;
-                const int x_chunk = grouped_x_box(PAIR, x_box(x_cols())) * kBlockK;
+                const int w_chunk = segs * (PAIR ? kTileRows : w.h) * kBlockK;
+                const int x_chunk = segs * grouped_x_box(PAIR, x_box(x_cols())) * kBlockK;
                 const uint64_t da1 = da0 - static_cast<uint64_t>((first_row() * kBlockK) >> 4);
                 for (int i = 0; i < nkb; ++i) {
                     if (!(ok = warp_wait<PAIR>(full_bar(s), ph, guard, kErrMmaWait))) break;
@@ -903,7 +970,70 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             while (step(ra) && step(rb)) {
             }
         }
-        if constexpr (FP4 && !PAIR) {
+        if constexpr (FP4 && FOLD) {
+            // Warps 2 and 3 take alternate stages and gather the words of every
+            // MMA row (W row r of segment a) and column, one by one.
+            const int seg_blocks = blocks / segs;
+            int s = 0, stage = 0;
+            uint32_t ph = 1u;
+            bool ok = true;
+            while (ok && walk.next(&w)) {
+                const uint32_t by_h = (65536u + w.h - 1) / w.h;  // exact quotients of numbers below 128
+                const uint8_t *ws[4], *xs[2];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int m = j * 32 + lane;
+                    int a = static_cast<int>((m * by_h) >> 16);
+                    const int r = min(w.w0 + m - a * w.h, p.n - 1);
+                    if (a >= segs) a = 0;
+                    ws[j] = p.w_scales + w.e * p.w_scale_stride +
+                            (static_cast<int64_t>(r >> 7) * blocks + a * seg_blocks) * kScaleBlock +
+                            (r & 31) * 16 + ((r >> 5) & 3) * 4;
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int c = j * 32 + lane;
+                    int a = c / (p.fold_x == 8 ? 8 : 16);
+                    const int r = w.row0 + min(c - a * p.fold_x, w.rows - 1);
+                    if (a >= segs) a = 0;
+                    xs[j] = p.x_scales +
+                            (static_cast<int64_t>(r >> 7) * blocks + a * seg_blocks) * kScaleBlock +
+                            (r & 31) * 16 + ((r >> 5) & 3) * 4;
+                }
+                for (int i = 0; i < nkb; ++i, ++stage) {
+                    if ((stage & 1) == warp - 2) {
+                        constexpr int kBlocks = kChunks * kSfPerChunk;
+                        uint32_t v[kBlocks][6];
+#pragma unroll
+                        for (int q = 0; q < kBlocks; ++q) {
+                            const int at = min(i * kBlocks + q, seg_blocks - 1) * kScaleBlock;
+#pragma unroll
+                            for (int j = 0; j < 6; ++j)
+                                v[q][j] = __ldg(reinterpret_cast<const uint32_t*>((j < 4 ? ws[j] : xs[j - 4]) + at));
+                        }
+                        if (stage >= stages && !(ok = warp_wait(empty_bar(s), ph, guard, kErrProducerWait)))
+                            break;
+                        const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
+#pragma unroll
+                        for (int q = 0; q < kBlocks; ++q) {
+                            sts_masked(wd + q * kScaleBlock, make_uint4(v[q][0], v[q][1], v[q][2], v[q][3]),
+                                       0xFFFFFFFFu);
+                            sts_masked(wd + kWsBytes + q * kScaleBlock, make_uint4(v[q][4], v[q][5], 0u, 0u),
+                                       0xFFFFFFFFu);
+                        }
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (elect_one()) mbar_arrive(full_bar(s));
+                        __syncwarp();
+                    }
+                    if (++s == stages) {
+                        s = 0;
+                        ph ^= 1u;
+                    }
+                }
+            }
+        }
+        if constexpr (FP4 && MODE == kStream) {
             // Warp 2 copies them: a block of W as it lies in memory (one
             // 16-byte copy per lane), X rows as 4-byte words gathered into the
             // block order.  It never waits for a copy: their completion arrives
@@ -994,13 +1124,46 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             if (p.alpha)
                 asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(alpha) : "l"(p.alpha + w.e * p.alpha_stride) : "memory");
             walk.ahead();
-            if (!warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait)) break;
+            bool ready = warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait);
+            if constexpr (FOLD) ready = epilogue_all(ready);  // the warps meet below: all or none
+            if (!ready) break;
             // The MMAs' commit reaches CTA 0 alone: pass it on.
             if (PAIR && rank == 0 && warp == 4 && lane == 0)
                 mbar_arrive_remote(at_rank(acc_full(b), 1));
             tc_fence_after_sync();
             const uint32_t taddr = tmem + b * p.acc_cols + (static_cast<uint32_t>(q * 32) << 16);
             __nv_bfloat16* row0 = p.y + static_cast<int64_t>(w.row0) * p.ldy;
+            if constexpr (FOLD) {
+                // Lane a h + r holds W row r in segment a: the columns of that
+                // segment go to shared memory, and the segments are added in
+                // order.
+                float* sums = reinterpret_cast<float*>(smem + p.out_off);
+                const int m = q * 32 + lane;
+                const uint32_t by_h = (65536u + w.h - 1) / w.h;  // exact quotients below 1,024 (h <= 64)
+                const int a = static_cast<int>((m * by_h) >> 16);
+                for (int i = 0; i < segs; ++i) {
+                    float v[8];
+                    for (int c = 0; c < p.fold_x; c += 8) {
+                        tmem_ld_x8(taddr + i * p.fold_x + c, v);
+                        if (i == a)
+#pragma unroll
+                            for (int t = 0; t < 8; ++t) sums[m * 17 + c + t] = v[t];
+                    }
+                }
+                tc_fence_before_sync();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(acc_empty(b));
+                epilogue_bar_sync();
+                for (int i = m; i < w.h * w.rows; i += 128) {
+                    const int t = static_cast<int>((i * by_h) >> 16);
+                    const int r = i - t * w.h;
+                    float sum = sums[r * 17 + t];
+                    for (int k = 1; k < segs; ++k) sum += sums[(k * w.h + r) * 17 + t];
+                    if (w.w0 + r < p.n) row0[t * p.ldy + w.w0 + r] = __float2bfloat16_rn(sum * alpha);
+                }
+                ++piece;
+                continue;
+            }
             // W rows of this warp's TMEM lanes, and those of them in the piece.
             const int n0 = w.w0 + rank * kTileRows - first_row() + q * 32;
             const int n_lo = PAIR ? n0 : w.w0;

@@ -10,34 +10,34 @@ using tinym::MxParams;
 
 // Tensor map of a stack of row-major uint8 matrices [experts, rows, cols].
 // chunks == 1: {cols, rows, experts} in boxes of [box_rows x 128 bytes].
-// chunks > 1 (cols % 128 == 0): {128, rows, cols / 128, experts}, a box is
-// `chunks` consecutive [box_rows x 128 bytes] tiles.  Past the end of any
-// dimension a box reads zeros.
+// chunks > 1: {128, rows, cols / 128, experts}, a box is `chunks` consecutive
+// [box_rows x 128 bytes] tiles (a partial last chunk is left out).
+// segs > 1: {128, rows, segs, cols / 128 / segs, experts}, each of the box's
+// tiles has box_rows rows of every segment, one segment after the other.
+// x: the X matrix, without the experts' dimension where that saves one.
+// Past the end of any dimension a box reads zeros.
 int encode_stack(const void* ptr, int64_t experts, int64_t rows, int64_t cols, int box_rows,
-                 int chunks, CUtensorMap* out) {
+                 int chunks, int segs, bool x, CUtensorMap* out) {
     auto encode = get_encode();
     if (!encode)
         return fail(TINYM_ERR_CUDA, "cuTensorMapEncodeTiled unavailable (%s)",
                     cudaGetErrorString(g_encode_err));
-    cuuint64_t dims[4], strides[3];
-    cuuint32_t box[4], estr[4] = {1, 1, 1, 1};
-    int rank = 0;
+    cuuint64_t dims[5], strides[4];
+    cuuint32_t box[5], estr[5] = {1, 1, 1, 1, 1};
+    int rank = 2;
+    auto dim = [&](int64_t size, int64_t stride, int b) {
+        dims[rank] = static_cast<cuuint64_t>(size);
+        strides[rank - 1] = static_cast<cuuint64_t>(stride);
+        box[rank++] = static_cast<cuuint32_t>(b);
+    };
     dims[0] = static_cast<cuuint64_t>(chunks > 1 ? kBlockK : cols);
     box[0] = kBlockK;
     dims[1] = static_cast<cuuint64_t>(rows);
     box[1] = static_cast<cuuint32_t>(box_rows);
     strides[0] = static_cast<cuuint64_t>(cols);
-    rank = 2;
-    if (chunks > 1) {
-        dims[rank] = static_cast<cuuint64_t>(cols / kBlockK);
-        box[rank] = static_cast<cuuint32_t>(chunks);
-        strides[rank - 1] = kBlockK;
-        ++rank;
-    }
-    dims[rank] = static_cast<cuuint64_t>(experts);
-    box[rank] = 1;
-    strides[rank - 1] = static_cast<cuuint64_t>(rows) * static_cast<cuuint64_t>(cols);
-    ++rank;
+    if (segs > 1) dim(segs, cols / segs, segs);
+    if (chunks > 1) dim(cols / kBlockK / segs, kBlockK, chunks);
+    if (!(x && segs > 1)) dim(experts, rows * cols, 1);
     const CUresult r = encode(out, CU_TENSOR_MAP_DATA_TYPE_UINT8, rank, const_cast<void*>(ptr), dims,
                               strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
                               CU_TENSOR_MAP_SWIZZLE_128B, TINYM_L2_PROMOTION,
@@ -121,16 +121,26 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
                     (long long)rows, (long long)experts, (long long)n);
     GroupedParams& p = g.prm;
     // A map per box height that the pieces can have.
-    const int chunks = !g.pair && p.chunked ? tinym::kStreamChunks : 1;
+    const int segs = std::max(1, p.fold);
+    const int chunks = g.pair || k_bytes < kBlockK ? 1 : tinym::kStreamChunks;
+    const bool tail = !g.pair && !p.chunked;
     tinym::GroupedMaps maps;
-    for (int i = g.pair ? tinym::kBlockUnits - 1 : 0; i < p.piece_units; ++i)
-        if ((st = encode_stack(w, experts, n, k_bytes, 8 * (i + 1), chunks, &maps.w[i])) != TINYM_OK)
+    for (int i = g.pair ? tinym::kBlockUnits - 1 : 0; i < p.piece_units; ++i) {
+        if ((st = encode_stack(w, experts, n, k_bytes, 8 * (i + 1), chunks, segs, false, &maps.w[i])) !=
+            TINYM_OK)
             return st;
+        if (tail && (st = encode_stack(w, experts, n, k_bytes, 8 * (i + 1), 1, 1, false,
+                                       &maps.w_tail[i])) != TINYM_OK)
+            return st;
+    }
+    const int64_t x_most = p.fold ? p.fold_x : std::min<int64_t>(p.tn, rows);
     for (int i = 0; i < 4; ++i) {
-        if ((st = encode_stack(x, 1, rows, k_bytes, tinym::grouped_x_box(g.pair, i), chunks,
-                               &maps.x[i])) != TINYM_OK)
+        const int box = tinym::grouped_x_box(g.pair, i);
+        if ((st = encode_stack(x, 1, rows, k_bytes, box, chunks, segs, true, &maps.x[i])) != TINYM_OK)
             return st;
-        if (tinym::grouped_x_box(g.pair, i) * (g.pair ? 2 : 1) >= std::min<int64_t>(p.tn, rows)) break;
+        if (tail && (st = encode_stack(x, 1, rows, k_bytes, box, 1, 1, true, &maps.x_tail[i])) != TINYM_OK)
+            return st;
+        if (box * (g.pair ? 2 : 1) >= x_most) break;
     }
     p.y = static_cast<__nv_bfloat16*>(y);
     p.ldy = ldy;
@@ -146,13 +156,13 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
     p.timeout_ns = kDefaultTimeoutNs;
     if ((st = pending_word(di, true, &p.err_host)) != TINYM_OK) return st;
 
-    static const void* const kFn[2][2] = {
-        {reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<false, false>),
-         reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<false, true>)},
-        {reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<true, false>),
-         reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<true, true>)}};
-    const void* fn = kFn[fp4 ? 1 : 0][g.pair ? 1 : 0];
-    const uint32_t bit = 1u << ((fp4 ? 2 : 0) + (g.pair ? 1 : 0));
+#define TINYM_GROUPED(F, M) reinterpret_cast<const void*>(&tinym::tinym_grouped_kernel<F, tinym::M>)
+    static const void* const kFn[2][3] = {
+        {TINYM_GROUPED(false, kStream), TINYM_GROUPED(false, kFold), TINYM_GROUPED(false, kPair)},
+        {TINYM_GROUPED(true, kStream), TINYM_GROUPED(true, kFold), TINYM_GROUPED(true, kPair)}};
+#undef TINYM_GROUPED
+    const void* fn = kFn[fp4 ? 1 : 0][g.mode];
+    const uint32_t bit = 1u << ((fp4 ? 3 : 0) + g.mode);
     if (!(g_grouped_attr[dev].load(std::memory_order_acquire) & bit)) {
         e = cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemLimit);
         if (e != cudaSuccess) return cuda_fail(e, "cudaFuncSetAttribute(MaxDynamicSharedMemorySize)");

@@ -92,7 +92,7 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
            "scale ring", p.sf_off, p.sf_stage);
     expect(p.w_off >= p.sf_off + p.stages * p.sf_stage && p.w_off % 1024 == 0, "W ring", p.w_off);
     expect(p.out_off >= p.w_off + p.stages * p.w_stage && p.out_off % 16 == 0, "output", p.out_off);
-    expect(p.bar_off >= p.out_off + 4u * tinym::kOutBytes && p.bar_off % 8 == 0, "barriers", p.bar_off);
+    expect(p.bar_off >= p.out_off + (p.fold ? tinym::kFoldOutBytes : 4 * tinym::kOutBytes) && p.bar_off % 8 == 0, "barriers", p.bar_off);
     expect(p.tab_off >= p.bar_off + 8u * (3 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
            p.tab_off);
     expect(p.tab_off + 8u * (p.experts + 1) + 1024 <= g.smem, "tables inside", p.tab_off, g.smem);
@@ -101,18 +101,32 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
     // X read at most 8 rows longer than the box
     expect(p.w_off + p.stages * p.w_stage + (g.pair ? 0 : 128 * 128) + 1024 <= g.smem, "W read inside", p.w_stage,
            g.smem);
-    expect(p.w_stage == p.piece_units * 8 * 128 * static_cast<int>(chunks), "W stage", p.w_stage);
+    const int segs = std::max(1, p.fold);
+    expect(p.w_stage == segs * p.piece_units * 8 * 128 * static_cast<int>(chunks), "W stage", p.w_stage);
+    expect((p.fold != 0) == (g.mode == tinym::kFold), "mode", p.fold, g.mode);
+    if (p.fold) {
+        expect(p.fold >= 2 && p.fold * p.piece_units <= 16 && p.fold * p.fold_x <= 64 && p.tn == 16 &&
+                   (p.fold_x == 8 || p.fold_x == 16) && p.fold_x >= std::min(p.rows, 16),
+               "folded rows and columns", p.fold, p.fold_x, p.piece_units);
+        expect(p.k_bytes % (128 * p.fold) == 0 && !p.blocked && !p.part_units, "segments", p.k_bytes, p.fold);
+        expect(p.x_stage == p.fold * p.fold_x * 128 * static_cast<int>(chunks), "folded X stage", p.x_stage);
+        expect(static_cast<int>(p.acc_cols) >= p.fold * p.fold_x && p.acc_cols % 16 == 0, "columns", p.acc_cols);
+        expect(p.bar_off >= p.out_off + 128 * 17 * 4, "folded sums", p.out_off, p.bar_off);
+        for (int h = 8; h <= p.piece_units * 8; h += 8)  // the kernels' quotients
+            for (int i = 0; i < 16 * h || i < 128; ++i)
+                expect(static_cast<int>((i * ((65536u + h - 1) / h)) >> 16) == i / h, "quotient", i, h);
+    }
     int box = 0;
-    while (box < 4 && tinym::grouped_x_box(g.pair, box) * (g.pair ? 2 : 1) < p.tn) ++box;
-    expect(box < 4 && tinym::grouped_x_box(g.pair, box) * 128 * static_cast<int>(chunks) <= p.x_stage, "X box", box,
+    while (box < 4 && tinym::grouped_x_box(g.pair, box) * (g.pair ? 2 : 1) < (p.fold ? p.fold_x : p.tn)) ++box;
+    expect(box < 4 && segs * tinym::grouped_x_box(g.pair, box) * 128 * static_cast<int>(chunks) <= p.x_stage, "X box", box,
            p.x_stage);
     expect(p.tn % 16 == 0 && p.tn >= 16 && p.tn <= 256 && (!g.pair || p.tn % 32 == 0) &&
                p.tn <= 128 * tinym::grouped_x_scale_blocks(g.pair),
            "tile width", p.tn);
-    expect(p.acc_cols >= static_cast<uint32_t>(p.tn) && p.tmem_cols <= 512 && (p.tmem_cols & (p.tmem_cols - 1)) == 0,
+    expect((p.fold || p.acc_cols >= static_cast<uint32_t>(p.tn)) && p.tmem_cols <= 512 && (p.tmem_cols & (p.tmem_cols - 1)) == 0,
            "tensor memory", p.acc_cols, p.tmem_cols);
-    expect((fp4 ? p.sf_col + 2 * tinym::kSfSlotCols : p.acc_cols + p.tn) <= p.tmem_cols &&
-               (!fp4 || (p.sf_col >= p.acc_cols + p.tn && p.sf_col % 4 == 0)),
+    expect((fp4 ? p.sf_col + 2 * tinym::kSfSlotCols : 2 * p.acc_cols) <= p.tmem_cols &&
+               (!fp4 || (p.sf_col >= 2 * p.acc_cols && p.sf_col % 4 == 0)),
            "scale columns", p.sf_col, p.tmem_cols);
     expect(g.grid >= 1 && (!g.pair || g.grid % 2 == 0), "grid", g.grid);
 }
@@ -140,14 +154,16 @@ int main() {
     std::srand(7);
     const int row_counts[] = {1, 2, 3, 15, 16, 17, 64, 65, 130, 257, 700};
     const int expert_counts[] = {1, 2, 5, 31, 32, 33, 64, 100};
-    const int ns[] = {1, 7, 8, 100, 129, 1000, 2050};
+    const int ns[] = {1, 7, 8, 100, 129, 1000, 2050, 6000};
     for (int rows : row_counts)
         for (int experts : expert_counts)
             for (int n : ns)
                 for (int mode = 0; mode < 5; ++mode)
                     for (int fp4 = 0; fp4 < 2; ++fp4) {
                         tinym::GroupedPlan g;
-                        const char* why = tinym::grouped_plan(fp4, rows, experts, n, 16 * (1 + std::rand() % 300),
+                        const char* why = tinym::grouped_plan(fp4, rows, experts, n,
+                                                              mode % 2 ? 128 * (1 + std::rand() % 48)
+                                                                       : 16 * (1 + std::rand() % 300),
                                                               mode == 4 ? 3 : 148, limit, &g);
                         expect(!why, "plan", rows, experts, n);
                         if (why) continue;

@@ -122,6 +122,13 @@ GROUPS = [
     ([257], 0, 1000, 1568),
     ([1, 700], 0, 384, 4128),
     ([0, 191, 193, 385], 0, 129, 96),
+    # few rows, K of whole 128-byte chunks: segments of K side by side in an MMA
+    ([1], 0, 2050, 6144),
+    ([16], 0, 1000, 1536),
+    ([7], 1, 640, 3584),
+    ([1, 0, 0, 2, 0, 1, 0, 0], 0, 1024, 2048),
+    ([0, 3, 17, 0, 1], 2, 500, 1024),
+    ([0] * 9 + [9], 0, 333, 768),
 ]
 
 
@@ -132,7 +139,8 @@ def test_fp8_gemm_grouped(cuda_device, counts, spare, n, k, per_expert):
 
     import candidate_kernel as ck
 
-    k += 16  # K a multiple of 16 only
+    if k % 256:
+        k += 16  # K a multiple of 16 only
     rows, e = sum(counts) + spare, len(counts)
     a, b = fp8((rows, k), 1), fp8((e, n, k), 2)
     alpha = torch.rand(e if per_expert else 1, generator=gen(3), device="cuda") / 64
@@ -345,24 +353,29 @@ def test_empty(cuda_device):
     assert ck.mxfp4_gemm(codes, scales, b, sb).shape == (0, 8)
 
 
-@pytest.mark.parametrize("rows", [24, 600])
-def test_rows_do_not_depend_on_the_split(cuda_device, rows):
-    """A row's result is the same alone, in a batch, in any group order and in
-    every run."""
+@pytest.mark.parametrize("rows", [4, 24, 600])
+def test_results_are_reproducible(cuda_device, rows):
+    """The same bits in every run, and for a row whatever groups the other rows
+    of the call are in."""
     import torch
 
     import candidate_kernel as ck
 
     n, k = 1100, 1536
     a, sa = quantized((rows, k), 1)
-    b, sb = quantized((2, n, k), 2)
-    off = offsets_of([rows // 3, rows - rows // 3])
-    y = ck.mxfp4_gemm_grouped(a, sa, b, sb, off)
+    b, sb = quantized((3, n, k), 2)
+    a8, b8 = fp8((rows, k), 3), fp8((3, n, k), 4)
+    one = torch.ones(1, device="cuda")
+    first = rows // 4
+    off = offsets_of([first, rows - first, 0])
+    y, y8 = ck.mxfp4_gemm_grouped(a, sa, b, sb, off), ck.fp8_gemm_grouped(a8, b8, one, off)
     for _ in range(3):
         assert torch.equal(y, ck.mxfp4_gemm_grouped(a, sa, b, sb, off))
-    all_first = ck.mxfp4_gemm(a, sa, b[0], sb[0])
-    assert torch.equal(y[:rows // 3], all_first[:rows // 3])
-    assert torch.equal(all_first[:1], ck.mxfp4_gemm(a[:1], sa[:1], b[0], sb[0]))
+        assert torch.equal(y8, ck.fp8_gemm_grouped(a8, b8, one, off))
+    for second in (1, rows // 2):
+        off = offsets_of([first, second, rows - first - second])
+        assert torch.equal(y[:first + second], ck.mxfp4_gemm_grouped(a, sa, b, sb, off)[:first + second])
+        assert torch.equal(y8[:first + second], ck.fp8_gemm_grouped(a8, b8, one, off)[:first + second])
 
 
 def test_captured_graph_replays_with_other_groups(cuda_device):
