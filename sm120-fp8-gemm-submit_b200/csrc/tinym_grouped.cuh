@@ -63,7 +63,7 @@ constexpr int kGrpMaxExperts = 1024;
 constexpr int kGrpBand = 8;          // row tiles walked together for each W tile (L2 reuse)
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
 constexpr int kStreamChunks = 4;     // 128-byte chunks of K in a stream stage
-constexpr int kGrpBars = 5;          // barriers beside the three per stage
+constexpr int kGrpBars = 5;          // barriers beside the two per stage
 constexpr int kFoldOutBytes = kTileRows * 17 * 4;  // folded: FP32 sums of 128 MMA rows x 16 X rows
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
@@ -353,7 +353,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.w_off = (std::max(p.w_off, front) + 1023u) & ~1023u;
         p.out_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
         p.bar_off = p.out_off + (p.fold ? kFoldOutBytes : 4 * kOutBytes);
-        p.tab_off = p.bar_off + 8u * (3 * stages + kGrpBars) + 8u;
+        p.tab_off = p.bar_off + 8u * (2 * stages + kGrpBars) + 8u;
         // The MMA's 128 W rows of the last chunk end inside the allocation.
         const uint32_t read_end = p.w_off + static_cast<uint32_t>(stages * p.w_stage) + kTileRows * kBlockK;
         return std::max(p.tab_off + tables, g.pair ? 0u : read_end) + 1024u;
@@ -522,12 +522,6 @@ __device__ __forceinline__ bool epilogue_all(bool ok) {
     return all != 0;
 }
 
-__device__ __forceinline__ void cp_async_4(uint32_t dst, const void* src) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
 // A lane's 16 bytes of the scale blocks of one pair stage.
 struct ScaleRegs {
     uint4 w[2], x[2][3];
@@ -548,14 +542,6 @@ __device__ __forceinline__ void sts_masked(uint32_t dst, const uint4& v, uint32_
                  "r"(v.y & mask), "r"(v.z & mask), "r"(v.w & mask)
                  : "memory");
 }
-// This thread's arrival on `bar` once its copies so far have landed.
-__device__ __forceinline__ void cp_async_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() {
-    asm volatile("cp.async.wait_all;" ::: "memory");
-}
-
 // 16 lanes x 16 columns as the fragments of 8 x 8 matrices: for columns 8 j ..
 // r[4 j], r[4 j + 1] are lane t / 4, columns 2 (t % 4) and + 1, the next two
 // lane t / 4 + 8.
@@ -647,11 +633,10 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const uint32_t bars = s_base + p.bar_off;
     auto full_bar = [&](int s) { return bars + 8u * s; };
     auto empty_bar = [&](int s) { return bars + 8u * (stages + s); };
-    auto sf_bar = [&](int s) { return bars + 8u * (2 * stages + s); };
-    auto acc_full = [&](int b) { return bars + 8u * (3 * stages + b); };
-    auto acc_empty = [&](int b) { return bars + 8u * (3 * stages + 2 + b); };
-    const uint32_t drain_bar = bars + 8u * (3 * stages + 4);
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (3 * stages + kGrpBars));
+    auto acc_full = [&](int b) { return bars + 8u * (2 * stages + b); };
+    auto acc_empty = [&](int b) { return bars + 8u * (2 * stages + 2 + b); };
+    const uint32_t drain_bar = bars + 8u * (2 * stages + 4);
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (2 * stages + kGrpBars));
     volatile uint32_t* abort_flag = tmem_slot + 1;
     int32_t* off = reinterpret_cast<int32_t*>(smem + p.tab_off);
     int32_t* prefix = off + p.experts + 1;
@@ -675,7 +660,6 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             // at CTA 0 of a pair the stage of CTA 1
             mbar_init(full_bar(s), 1 + (FP4 ? 1 : 0) + (PAIR && rank == 0 ? 1 : 0));
             mbar_init(empty_bar(s), 1);
-            mbar_init(sf_bar(s), 32);  // the lanes of the scale warp
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(acc_full(b), 1);
@@ -691,15 +675,27 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     // dependent launch); no global memory is read before it has completed.
     grid_dependency_wait();
     grid_launch_dependents();
-    if (warp == 2) grouped_tables(p, off, prefix, lane);
-    tc_fence_before_sync();
-    __syncthreads();
-    if constexpr (PAIR) {  // the other CTA's barriers exist before anything arrives on them
+    if (warp == 0) grouped_tables(p, off, prefix, lane);
+    uint32_t tmem = 0u;
+    if constexpr (PAIR) {
+        tc_fence_before_sync();
+        __syncthreads();
+        // the other CTA's barriers exist before anything arrives on them
         cluster_arrive_release();
         cluster_wait_acquire();
+        tc_fence_after_sync();
+        tmem = *tmem_slot;
+    } else if (warp == 0) {
+        // The producer made the barriers and the tables itself: it loads the
+        // first stages while the others come to the barrier.
+        __syncwarp();
+        asm volatile("barrier.cta.arrive 2, 256;" ::: "memory");
+    } else {
+        tc_fence_before_sync();
+        asm volatile("barrier.cta.sync 2, 256;" ::: "memory");
+        tc_fence_after_sync();
+        tmem = *tmem_slot;
     }
-    tc_fence_after_sync();
-    const uint32_t tmem = *tmem_slot;
 
     GroupedAhead<PAIR> walk(p, off, prefix, blockIdx.x / kCtas, gridDim.x / kCtas);
     GroupedPiece w;
@@ -970,147 +966,92 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             while (step(ra) && step(rb)) {
             }
         }
-        if constexpr (FP4 && FOLD) {
-            // Warps 2 and 3 take alternate stages and gather the words of every
-            // MMA row (W row r of segment a) and column, one by one.
+        if constexpr (FP4 && !PAIR) {
+            // Warps 2 and 3 take alternate stages, each with the scales of its
+            // next one in registers.  X words, and folded the W words of every
+            // MMA row (W row r of segment a), are gathered one by one; else a
+            // W block is stored as it is.  (4-byte cp.async took ~50 cycles
+            // each: 0.7 us a stage of 32 X rows or more.)
+            constexpr int kBlocks = kChunks * kSfPerChunk;
             const int seg_blocks = blocks / segs;
-            int s = 0, stage = 0;
+            uint32_t v[kBlocks][6];
+            const uint8_t* ws[FOLD ? 4 : 1] = {};
+            const uint8_t* xs[2] = {};
+            int i = warp - 2, first = 0;
+            // The scale word of 128-column group 0 of row r (of a segment).
+            auto word_at = [&](const uint8_t* base, int r, int a) {
+                return base + (static_cast<int64_t>(r >> 7) * blocks + a * seg_blocks) * kScaleBlock +
+                       (r & 31) * 16 + ((r >> 5) & 3) * 4;
+            };
+            auto enter = [&]() {  // a piece
+                const uint8_t* base = p.w_scales + w.e * p.w_scale_stride;
+                if constexpr (FOLD) {
+                    const uint32_t by_h = (65536u + w.h - 1) / w.h;  // exact quotients below 128
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int m = j * 32 + lane, a = static_cast<int>((m * by_h) >> 16);
+                        ws[j] = word_at(base, min(w.w0 + m - a * w.h, p.n - 1), a < segs ? a : 0);
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const int c = j * 32 + lane, a = c / (p.fold_x == 8 ? 8 : 16);
+                        xs[j] = word_at(p.x_scales, w.row0 + min(c - a * p.fold_x, w.rows - 1),
+                                        a < segs ? a : 0);
+                    }
+                } else {
+                    ws[0] = base + static_cast<int64_t>(w.w0 >> 7) * blocks * kScaleBlock + lane * 16;
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        xs[j] = word_at(p.x_scales, w.row0 + min(j * 32 + lane, w.rows - 1), 0);
+                }
+            };
+            bool more = walk.next(&w);
+            if (more) enter();
+            auto fetch = [&]() {  // this warp's next stage, if there is one
+                while (more && i >= nkb) {
+                    i -= nkb;
+                    if ((more = walk.next(&w))) enter();
+                }
+                if (!more) return;
+                first = i * kBlocks;
+                i += 2;
+#pragma unroll
+                for (int q = 0; q < kBlocks; ++q) {
+                    const int64_t at = static_cast<int64_t>(min(first + q, seg_blocks - 1)) * kScaleBlock;
+                    if constexpr (FOLD) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+                            v[q][j] = __ldg(reinterpret_cast<const uint32_t*>(ws[j] + at));
+                    } else {
+                        const uint4 o = __ldg(reinterpret_cast<const uint4*>(ws[0] + at));
+                        v[q][0] = o.x, v[q][1] = o.y, v[q][2] = o.z, v[q][3] = o.w;
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j)
+                        v[q][4 + j] = __ldg(reinterpret_cast<const uint32_t*>(xs[j] + at));
+                }
+            };
+            fetch();
+            int s = warp - 2;
             uint32_t ph = 1u;
-            bool ok = true;
-            while (ok && walk.next(&w)) {
-                const uint32_t by_h = (65536u + w.h - 1) / w.h;  // exact quotients of numbers below 128
-                const uint8_t *ws[4], *xs[2];
+            while (more) {
+                if (!warp_wait(empty_bar(s), ph, guard, kErrProducerWait)) break;
+                const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int m = j * 32 + lane;
-                    int a = static_cast<int>((m * by_h) >> 16);
-                    const int r = min(w.w0 + m - a * w.h, p.n - 1);
-                    if (a >= segs) a = 0;
-                    ws[j] = p.w_scales + w.e * p.w_scale_stride +
-                            (static_cast<int64_t>(r >> 7) * blocks + a * seg_blocks) * kScaleBlock +
-                            (r & 31) * 16 + ((r >> 5) & 3) * 4;
+                for (int q = 0; q < kBlocks; ++q) {
+                    const uint32_t mask = FOLD ? 0xFFFFFFFFu : block_mask(first + q);
+                    sts_masked(wd + q * kScaleBlock, make_uint4(v[q][0], v[q][1], v[q][2], v[q][3]), mask);
+                    sts_masked(wd + kWsBytes + q * kScaleBlock, make_uint4(v[q][4], v[q][5], 0u, 0u), mask);
                 }
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const int c = j * 32 + lane;
-                    int a = c / (p.fold_x == 8 ? 8 : 16);
-                    const int r = w.row0 + min(c - a * p.fold_x, w.rows - 1);
-                    if (a >= segs) a = 0;
-                    xs[j] = p.x_scales +
-                            (static_cast<int64_t>(r >> 7) * blocks + a * seg_blocks) * kScaleBlock +
-                            (r & 31) * 16 + ((r >> 5) & 3) * 4;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (elect_one()) mbar_arrive(full_bar(s));
+                __syncwarp();
+                if ((s += 2) >= stages) {
+                    s -= stages;
+                    ph ^= 1u;
                 }
-                for (int i = 0; i < nkb; ++i, ++stage) {
-                    if ((stage & 1) == warp - 2) {
-                        constexpr int kBlocks = kChunks * kSfPerChunk;
-                        uint32_t v[kBlocks][6];
-#pragma unroll
-                        for (int q = 0; q < kBlocks; ++q) {
-                            const int at = min(i * kBlocks + q, seg_blocks - 1) * kScaleBlock;
-#pragma unroll
-                            for (int j = 0; j < 6; ++j)
-                                v[q][j] = __ldg(reinterpret_cast<const uint32_t*>((j < 4 ? ws[j] : xs[j - 4]) + at));
-                        }
-                        if (stage >= stages && !(ok = warp_wait(empty_bar(s), ph, guard, kErrProducerWait)))
-                            break;
-                        const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
-#pragma unroll
-                        for (int q = 0; q < kBlocks; ++q) {
-                            sts_masked(wd + q * kScaleBlock, make_uint4(v[q][0], v[q][1], v[q][2], v[q][3]),
-                                       0xFFFFFFFFu);
-                            sts_masked(wd + kWsBytes + q * kScaleBlock, make_uint4(v[q][4], v[q][5], 0u, 0u),
-                                       0xFFFFFFFFu);
-                        }
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (elect_one()) mbar_arrive(full_bar(s));
-                        __syncwarp();
-                    }
-                    if (++s == stages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
-                }
-            }
-        }
-        if constexpr (FP4 && MODE == kStream) {
-            // Warp 2 copies them: a block of W as it lies in memory (one
-            // 16-byte copy per lane), X rows as 4-byte words gathered into the
-            // block order.  It never waits for a copy: their completion arrives
-            // on sf_bar, where warp 3 waits, makes them visible to the tensor
-            // core's copies and passes them on.
-            int s = 0;
-            bool ok = true;
-            if (warp == 2) {
-                constexpr int kGroups = 2;  // of 32 X rows
-                uint32_t ph = 1u;
-                while (ok && walk.next(&w)) {
-                    const uint8_t* ws = p.w_scales + w.e * p.w_scale_stride +
-                                        static_cast<int64_t>(w.w0 >> 7) * blocks * kScaleBlock + lane * 16;
-                    const uint8_t* xs[kGroups];
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) {
-                        const int r = w.row0 + min(g * 32 + lane, w.rows - 1);
-                        xs[g] = p.x_scales + static_cast<int64_t>(r >> 7) * blocks * kScaleBlock +
-                                (r & 31) * 16 + ((r >> 5) & 3) * 4;
-                    }
-                    for (int i = 0; i < nkb; ++i) {
-                        if (!(ok = warp_wait(empty_bar(s), ph, guard, kErrProducerWait))) break;
-                        const uint32_t wd = sf_ring + s * p.sf_stage + lane * 16;
-                        const uint32_t xd = wd + kWsBytes;
-                        const int b0 = i * kChunks * kSfPerChunk;
-                        const bool whole = b0 + kChunks * kSfPerChunk < blocks + (tail == 0 ? 1 : 0);
-                        if (whole) {
-#pragma unroll
-                            for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
-                                const int64_t at = static_cast<int64_t>(b0 + q) * kScaleBlock;
-                                cp_async_16(wd + q * kScaleBlock, ws + at);
-#pragma unroll
-                                for (int g = 0; g < kGroups; ++g)
-                                    if (g * 32 < w.rows)
-                                        cp_async_4(xd + q * kScaleBlock + g * 4, xs[g] + at);
-                            }
-                            cp_async_arrive(sf_bar(s));
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < kChunks * kSfPerChunk; ++q) {
-                                const uint32_t mask = block_mask(b0 + q);
-                                const int64_t at = static_cast<int64_t>(min(b0 + q, blocks - 1)) * kScaleBlock;
-                                sts_masked(wd + q * kScaleBlock, __ldg(reinterpret_cast<const uint4*>(ws + at)),
-                                           mask);
-#pragma unroll
-                                for (int g = 0; g < kGroups; ++g)
-                                    if (g * 32 < w.rows) {
-                                        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>(xs[g] + at));
-                                        asm volatile("st.shared.u32 [%0], %1;" ::"r"(xd + q * kScaleBlock + g * 4),
-                                                     "r"(v & mask)
-                                                     : "memory");
-                                    }
-                            }
-                            mbar_arrive(sf_bar(s));
-                        }
-                        if (++s == stages) {
-                            s = 0;
-                            ph ^= 1u;
-                        }
-                    }
-                }
-                cp_async_wait_all();  // none is in flight when shared memory is released
-            } else {
-                uint32_t ph = 0u;
-                while (ok && walk.next(&w)) {
-                    for (int i = 0; i < nkb; ++i) {
-                        if (!(ok = warp_wait(sf_bar(s), ph, guard, kErrConsumerWait))) break;
-                        fence_proxy_async_smem();
-                        __syncwarp();
-                        if (elect_one()) mbar_arrive(full_bar(s));
-                        __syncwarp();
-                        if (++s == stages) {
-                            s = 0;
-                            ph ^= 1u;
-                        }
-                    }
-                }
+                fetch();
             }
         }
     } else {
@@ -1202,24 +1143,36 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                                           pack_bf16(f[4], f[5], alpha), pack_bf16(f[6], f[7], alpha));
                     }
                 __syncwarp();
+                if (p.wide_y) {
 #pragma unroll
-                for (int k = 0; k < kCols / 8; ++k) {
-                    const int r = 8 * k + (lane >> 2), ch = lane & 3;
-                    const int n = n0 + ch * 8;
-                    const uint4 o = *reinterpret_cast<const uint4*>(
-                        buf + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16));
-                    if (c + r < w.rows && n >= n_lo && n < n_hi) {
-                        __nv_bfloat16* dst = row0 + (c + r) * p.ldy + n;
-                        if (p.wide_y && n + 8 <= n_hi) {
-                            *reinterpret_cast<uint4*>(dst) = o;
-                        } else {
-                            const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
+                    for (int k = 0; k < kCols / 8; ++k) {
+                        const int r = 8 * k + (lane >> 2), ch = lane & 3;
+                        const int n = n0 + ch * 8;
+                        const uint4 o = *reinterpret_cast<const uint4*>(
+                            buf + r * 64 + ((ch ^ ((r >> 1) & 3)) * 16));
+                        if (c + r < w.rows && n >= n_lo && n < n_hi) {
+                            __nv_bfloat16* dst = row0 + (c + r) * p.ldy + n;
+                            if (n + 8 <= n_hi) {
+                                *reinterpret_cast<uint4*>(dst) = o;
+                            } else {
+                                const uint32_t ow[4] = {o.x, o.y, o.z, o.w};
 #pragma unroll
-                            for (int i = 0; i < 8; ++i)
-                                if (n + i < n_hi)
-                                    reinterpret_cast<uint16_t*>(dst)[i] =
-                                        static_cast<uint16_t>(ow[i / 2] >> (16 * (i & 1)));
+                                for (int i = 0; i < 8; ++i)
+                                    if (n + i < n_hi)
+                                        reinterpret_cast<uint16_t*>(dst)[i] =
+                                            static_cast<uint16_t>(ow[i / 2] >> (16 * (i & 1)));
+                            }
                         }
+                    }
+                } else {
+                    // Y's rows do not start on 16 bytes: one value per lane,
+                    // 64 bytes of a row per warp.
+                    const int n = n0 + lane;
+#pragma unroll
+                    for (int r = 0; r < kCols; ++r) {
+                        if (c + r < w.rows && n >= n_lo && n < n_hi)
+                            row0[(c + r) * p.ldy + n] = *reinterpret_cast<const __nv_bfloat16*>(
+                                buf + r * 64 + (((lane >> 3) ^ ((r >> 1) & 3)) * 16) + (lane & 7) * 2);
                     }
                 }
                 __syncwarp();

@@ -93,7 +93,7 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
     expect(p.w_off >= p.sf_off + p.stages * p.sf_stage && p.w_off % 1024 == 0, "W ring", p.w_off);
     expect(p.out_off >= p.w_off + p.stages * p.w_stage && p.out_off % 16 == 0, "output", p.out_off);
     expect(p.bar_off >= p.out_off + (p.fold ? tinym::kFoldOutBytes : 4 * tinym::kOutBytes) && p.bar_off % 8 == 0, "barriers", p.bar_off);
-    expect(p.tab_off >= p.bar_off + 8u * (3 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
+    expect(p.tab_off >= p.bar_off + 8u * (2 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
            p.tab_off);
     expect(p.tab_off + 8u * (p.experts + 1) + 1024 <= g.smem, "tables inside", p.tab_off, g.smem);
     const uint32_t chunks = g.pair ? 1 : tinym::kStreamChunks;
