@@ -62,7 +62,6 @@ constexpr int kGrpThreads = 256;     // warp 0 TMA, 1 MMA, 2-3 scales, 4-7 epilo
 constexpr int kGrpMaxExperts = 1024;
 constexpr int kGrpBand = 8;          // row tiles walked together for each W tile (L2 reuse)
 constexpr int kScaleBlock = 512;     // scale bytes of 128 rows x 4 scales
-constexpr int kStreamChunks = 4;     // 128-byte chunks of K in a stream stage
 constexpr int kGrpBars = 5;          // barriers beside the two per stage
 constexpr int kFoldOutBytes = kTileRows * 17 * 4;  // folded: FP32 sums of 128 MMA rows x 16 X rows
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
@@ -121,6 +120,15 @@ __host__ __device__ constexpr int grouped_x_box(bool pair, int i) { return (pair
 constexpr uint32_t kGrpZeroRest = 1u;  // rows of no group are written as zeros
 
 constexpr int kBlockUnits = kTileRows / 8;  // 8-row units of a 128-row block
+
+enum GroupedMode { kStream, kFold, kPair };
+// 128-byte chunks of K in a stage: one for a pair's 512 cycles of MMAs, four
+// where the bytes of W bind (two took 4-6 % longer on decode batches), two for
+// the smallest calls, whose first MMA waits for a whole stage (four took 5 %
+// longer at 1 x 5120 x 6144).
+__host__ __device__ constexpr int grouped_chunks(GroupedMode m) {
+    return m == kPair ? 1 : m == kFold ? 2 : 4;
+}
 
 // 128-row scale blocks of the X rows of a tile: stream tiles have at most 128 rows.
 __host__ __device__ constexpr int grouped_x_scale_blocks(bool pair) { return pair ? 2 : 1; }
@@ -250,7 +258,6 @@ struct GroupedAhead {
 };
 
 // How a call is cut.
-enum GroupedMode { kStream, kFold, kPair };
 struct GroupedPlan {
     GroupedMode mode;
     bool pair;  // mode == kPair
@@ -276,7 +283,6 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     p.n = static_cast<int32_t>(n);
     p.k_bytes = static_cast<int32_t>(k_bytes);
     const int64_t k_chunks = (k_bytes + kBlockK - 1) / kBlockK;
-    const int chunks = g.pair ? 1 : kStreamChunks;  // of a stage
     // Bytes in front of the W ring that an MMA may read: a piece that starts
     // inside a scale block stands that many rows into the MMA's rows.
     const uint32_t front = fp4 && !g.pair ? kTileRows * kBlockK : 0;
@@ -327,7 +333,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
             x_rows = p.fold * p.fold_x;
             p.acc_cols = static_cast<uint32_t>((x_rows + 15) / 16 * 16);
         }
-        p.x_stage = x_rows * chunks * kBlockK;
+        p.x_stage = x_rows * grouped_chunks(g.mode) * kBlockK;
         p.sf_col = 2 * p.acc_cols;
         p.tmem_cols = 32;
         while (p.tmem_cols < 2 * p.acc_cols + (fp4 ? 2 * kSfSlotCols : 0)) p.tmem_cols *= 2;
@@ -337,6 +343,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     p.by_parts = FastDiv::make(static_cast<uint32_t>(
         p.part_units ? (kBlockUnits + p.part_units - 1) / p.part_units : 1));
     for (int i = 0; i < kGrpBand; ++i) p.by_width[i] = FastDiv::make(static_cast<uint32_t>(i + 1));
+    const int chunks = grouped_chunks(g.mode);
     p.w_stage = std::max(1, p.fold) * p.piece_units * chunks * 1024;
     if (fp4) p.sf_stage = chunks * 2 * (1 + grouped_x_scale_blocks(g.pair)) * kScaleBlock;
     const int64_t max_items = (groups + rows / p.tn) * p.units;
@@ -617,7 +624,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     constexpr bool PAIR = MODE == kPair, FOLD = MODE == kFold;
     using Ops = Tc<PAIR ? 2 : 1>;
     constexpr int kCtas = PAIR ? 2 : 1;
-    constexpr int kChunks = PAIR ? 1 : kStreamChunks;  // 128-byte chunks of K per stage
+    constexpr int kChunks = grouped_chunks(MODE);  // 128-byte chunks of K per stage
     constexpr int kMmaK = 32;              // bytes of K per MMA (32 E4M3 or 64 E2M1 elements)
     constexpr int kSfPerChunk = 2;         // MXFP4: scale blocks (128 elements) per chunk
     constexpr int kXsBlocks = grouped_x_scale_blocks(PAIR);
@@ -650,9 +657,17 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const int nkb = (k_chunks + kChunks - 1) / kChunks;
     auto at_rank = [&](uint32_t addr, int r) { return PAIR ? dsmem_map(addr, r) : addr; };
 
-    if (threadIdx.x == 96) {  // the maps that the first stage is likely to use
-        tma_prefetch_desc(&maps.w[p.piece_units - 1]);
-        tma_prefetch_desc(&maps.x[0]);
+    if (warp == 3) {
+        // What the producer will need first: the maps that the first stage is
+        // likely to use, and the parameters (a miss of the constant cache
+        // costs some hundred cycles, and the walk would take them one by one).
+        if (lane == 0) {
+            tma_prefetch_desc(&maps.w[p.piece_units - 1]);
+            tma_prefetch_desc(&maps.x[0]);
+        }
+        asm volatile("" ::"r"(p.rows), "r"(p.units), "r"(p.stages), "r"(p.sf_off), "r"(p.by_grid.mul),
+                     "r"(p.by_band.mul), "r"(p.by_width[2].mul), "r"(p.by_width[7].mul), "r"(p.flags)
+                     : "memory");
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {

@@ -122,7 +122,7 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
     GroupedParams& p = g.prm;
     // A map per box height that the pieces can have.
     const int segs = std::max(1, p.fold);
-    const int chunks = g.pair || k_bytes < kBlockK ? 1 : tinym::kStreamChunks;
+    const int chunks = g.pair || k_bytes < kBlockK ? 1 : tinym::grouped_chunks(g.mode);
     const bool tail = !g.pair && !p.chunked;
     tinym::GroupedMaps maps;
     for (int i = g.pair ? tinym::kBlockUnits - 1 : 0; i < p.piece_units; ++i) {

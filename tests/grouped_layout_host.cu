@@ -96,7 +96,7 @@ void check_plan(const tinym::GroupedPlan& g, bool fp4, uint32_t limit) {
     expect(p.tab_off >= p.bar_off + 8u * (2 * p.stages + tinym::kGrpBars) + 8u && p.tab_off % 4 == 0, "tables",
            p.tab_off);
     expect(p.tab_off + 8u * (p.experts + 1) + 1024 <= g.smem, "tables inside", p.tab_off, g.smem);
-    const uint32_t chunks = g.pair ? 1 : tinym::kStreamChunks;
+    const uint32_t chunks = tinym::grouped_chunks(g.mode);
     // every W read is 128 rows of a chunk that starts inside its stage, every
     // X read at most 8 rows longer than the box
     expect(p.w_off + p.stages * p.w_stage + (g.pair ? 0 : 128 * 128) + 1024 <= g.smem, "W read inside", p.w_stage,
