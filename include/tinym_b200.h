@@ -326,6 +326,14 @@ TINYM_API int tinym_fp8_gemm_grouped(const void* x, const void* w, void* y, int6
                                      const int32_t* offsets_dev, const float* alpha_dev,
                                      int32_t alpha_count, uint32_t flags, void* stream);
 
+/* Failure-detection self-test of the grouped kernel, as
+ * tinym_selftest_wait_timeout: no copy is issued, so every wait runs out after
+ * timeout_ns and is reported; Y is unspecified. */
+TINYM_API int tinym_selftest_grouped_timeout(const void* x, const void* w, void* y, int64_t rows,
+                                             int64_t experts, int64_t n, int64_t k,
+                                             const int32_t* offsets_dev, uint64_t timeout_ns,
+                                             void* stream);
+
 /* ------------------------------------------------------------------------
  * MXFP4: E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), one
  * E8M0 scale byte s (2^(s - 127); 255 = NaN) per 32 consecutive columns.

@@ -16,33 +16,39 @@
 // groups' row tiles in shared memory and every role of the CTA walks the same
 // list of pieces (group, row tile, W rows).
 //
-//  * Stream pieces, for few rows per group, where the time is
-//    W's bytes: the W rows of all non-empty groups are laid end to end in
-//    units of 8 rows and each CTA takes an equal, contiguous share of them,
-//    walked in pieces of at most 128 rows with the whole of K.  The shares
-//    differ by at most one unit, so every SM streams the same number of bytes
-//    whatever the groups are, with no split of K, no workspace and one fixed
-//    order of every sum.  A stage is 512 bytes of K
-//    (256 bytes took 10 % longer on one-token calls, 4 % on decode batches).
-//  * Folded stream pieces (FOLD), for so little work that a CTA's share is at
-//    most 64 W rows and a tile at most 16 X rows.  An MMA costs ~45 cycles to
+//  * Stream pieces, for few rows per group, where the time is W's bytes: the W
+//    rows of all non-empty groups are laid end to end in units of 8 rows and
+//    each CTA takes an equal, contiguous share of them, walked in pieces of at
+//    most 128 rows with the whole of K.  The shares differ by at most one
+//    unit, so every SM streams the same number of bytes whatever the groups
+//    are, with no split of K over CTAs, no workspace and one fixed order of
+//    every sum.  28 experts of 2048 x 5120 E4M3 with 128 rows: 51 us, 5.8 TB/s
+//    (89 % of the measured copy); 60 of 2000 x 4096 MXFP4 with 256 rows: 45 us,
+//    5.8 TB/s.
+//  * Folded stream pieces, for so little work that a CTA's share is at most 64
+//    W rows and a tile at most 16 X rows.  An MMA costs ~45 cycles to
 //    issue whether 30 or 128 of its rows are used, and a share takes K / 32
 //    bytes of them.  So K is cut into S segments that stand side by side in
 //    one MMA: A row a h + r is W row r in segment a, B column b x + t is X row
 //    t in segment b, the S diagonal blocks of the product are the segments'
-//    sums, and the epilogue adds them in order: a S-th of the instructions.
+//    sums, and the epilogue adds them in order: an S-th of the instructions
+//    (1 x 5120 x 6144: E4M3 11.2 -> 9.2 us, MXFP4 8.4 -> 7.2 us).
 //  * Pair pieces, for many rows per group, where the time is the
 //    tensor core's: two CTAs (cta_group::2) compute 256 W rows x up to 256 X
 //    rows, 128 bytes of K a stage.  Each loads its 128 W rows and half of the
 //    X rows, so a CTA moves 256 rows of K for 128 x 256 sums where one CTA
 //    alone would move 384: the L2 feeds the SMs at ~42 bytes/clk/SM here,
-//    which held single-CTA 128 x 256 tiles at 1.77 PFLOP/s of E4M3.
+//    which held single-CTA 128 x 256 tiles at 1.77 PFLOP/s of E4M3.  Measured:
+//    E4M3 2.65 PFLOP/s in a burst and 2.4 under the power cap (8192 x 5120 x
+//    6144), MXFP4 4.7 and 4.3 (4096 x 16384 x 5120); both sit at 1,000 W with
+//    the SM clock at 1.1 - 1.4 GHz.
 //
 // MXFP4 scales reach TMEM by tcgen05.cp in blocks of 128 rows x 4 scales
 // (lane i, column j = row 32 j + i), the order in which they lie in memory.
-// W row r is therefore always MMA row r % 128: a stream piece never crosses a
-// multiple of 128 rows, and its block is copied as it is.  X tiles start at
-// any row; their scale words are gathered into the block order.
+// W row r is therefore always MMA row r % 128 (but in folded pieces): a stream
+// piece never crosses a multiple of 128 rows, and its block is copied as it
+// is.  X tiles start at any row; their scale words are gathered into the block
+// order.
 //
 // A stage's W and X are one box each, [chunks of 128 B][rows][128 B]: a bulk
 // copy costs its issuing thread ~90 cycles whatever its size (measured), so
@@ -117,6 +123,7 @@ struct GroupedMaps {
     CUtensorMap x_tail[4];
 };
 __host__ __device__ constexpr int grouped_x_box(bool pair, int i) { return (pair ? 16 : 8) << i; }
+constexpr uint32_t kGrpNoLoads = 2u;   // self-test: no copy is issued, every wait runs out
 constexpr uint32_t kGrpZeroRest = 1u;  // rows of no group are written as zeros
 
 constexpr int kBlockUnits = kTileRows / 8;  // 8-row units of a 128-row block
@@ -729,7 +736,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         const uint64_t pol_x = l2_policy_evict_last();
         int s = 0, issued = 0;
         uint32_t ph = 1u;  // the first pass over the ring does not wait
-        bool ok = true;
+        bool ok = !(p.flags & kGrpNoLoads);
         while (ok && walk.next(&w)) {
             const int cols = x_cols();
             const int xi = x_box(cols);

@@ -129,6 +129,7 @@ GROUPS = [
     ([1, 0, 0, 2, 0, 1, 0, 0], 0, 1024, 2048),
     ([0, 3, 17, 0, 1], 2, 500, 1024),
     ([0] * 9 + [9], 0, 333, 768),
+    ([0] * 1000 + [3, 0, 70, 1], 0, 24, 160),
 ]
 
 
@@ -252,6 +253,25 @@ def test_mxfp4_quantize_special_values(cuda_device):
     assert torch.equal(back.isnan(), mx_values(codes, scales).isnan())
     keep = ~back.isnan()
     assert torch.equal(back[keep].double(), mx_values(codes, scales)[keep])
+
+
+@pytest.mark.parametrize("dtype_name", ["bfloat16", "float32"])
+def test_mxfp4_dequantize_every_code_and_scale(cuda_device, dtype_name):
+    """Exact wherever the type can hold the value (6 * 2^127 becomes infinite)."""
+    import torch
+
+    import candidate_kernel as ck
+
+    dtype = getattr(torch, dtype_name)
+    codes = torch.arange(256, device="cuda").to(torch.uint8).reshape(16, 16).repeat(16, 8)  # [256, 128]
+    scales = torch.arange(256, device="cuda").to(torch.uint8)  # row r: scale r
+    rows = scales[:, None].expand(256, 8)
+    blocked = rows.reshape(2, 4, 32, 2, 4).permute(0, 3, 2, 1, 4).reshape(2, 2, 512).contiguous()
+    got = ck.mxfp4_dequantize(codes, blocked, dtype)
+    want = mx_values(codes, blocked).to(dtype)
+    nan = want.isnan()
+    assert torch.equal(got.isnan(), nan) and nan.any() and want.isinf().any()
+    assert torch.equal(got[~nan], want[~nan])
 
 
 def test_nan_stays_in_its_row(cuda_device):
@@ -432,6 +452,34 @@ def test_two_streams_at_once(cuda_device):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(w, y) for y in g)
+
+
+@pytest.mark.parametrize("rows,experts,n,k", [(2, 2, 1000, 2048), (40, 4, 300, 1024), (700, 2, 600, 1024)])
+def test_waits_that_run_out_are_reported(cuda_device, rows, experts, n, k):
+    """Folded, stream and pair kernel: without copies every wait ends after its
+    limit, the next call raises, and the one after that is right again."""
+    import torch
+
+    import candidate_kernel as ck
+    import tinym_b200 as t
+
+    a, b = fp8((rows, k), 1), fp8((experts, n, k), 2)
+    one, off = torch.ones(1, device="cuda"), offsets_of([1] * (experts - 1) + [rows - experts + 1])
+    want = ck.fp8_gemm_grouped(a, b, one, off)
+    torch.cuda.synchronize()
+    assert t.device_status(clear=True) == 0
+    y = torch.empty_like(want)
+    lib = t.capi()
+    st = lib.tinym_selftest_grouped_timeout(a.data_ptr(), b.data_ptr(), y.data_ptr(), rows, experts, n, k,
+                                            off.data_ptr(), 2_000_000,
+                                            torch.cuda.current_stream().cuda_stream)
+    assert st == 0, lib.tinym_last_error()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="TINYM_ERR_DEVICE_TIMEOUT"):
+        ck.fp8_gemm_grouped(a, b, one, off)
+    assert torch.equal(ck.fp8_gemm_grouped(a, b, one, off), want)
+    assert t.device_status(clear=True) != 0
+    assert t.device_status() == 0 and t.pending_errors() == 0
 
 
 def test_refusals(cuda_device):

@@ -62,6 +62,11 @@ def test_mxfp4_gemm_refusals():
     assert _lib().tinym_mxfp4_gemm(P, P, P, P, P, 64, 0, 64, 64, None, None) == 1
 
 
+def test_selftest_rejects_bad_timeout():
+    for ns in (0, 10 ** 11):
+        assert _lib().tinym_selftest_grouped_timeout(P, P, P, 4, 2, 64, 64, P, ns, None) == 1
+
+
 @pytest.mark.parametrize("batch,rows,k,want", [
     (1, 1, 32, 512), (1, 128, 128, 512), (1, 129, 128, 1024), (1, 1, 160, 1024), (3, 200, 6144, 3 * 2 * 48 * 512),
 ])
