@@ -64,6 +64,17 @@ def row_scales(scales, rows, cols):
     return scales[r // 128, c // 4, (r % 32) * 16 + (r // 32 % 4) * 4 + c % 4]
 
 
+def scale_block(byte):
+    """Row scales [R, C] in the blocked layout."""
+    import torch
+
+    r, c = byte.shape
+    full = torch.zeros(-(-r // 128) * 128, -(-c // 4) * 4, dtype=torch.uint8, device=byte.device)
+    full[:r, :c] = byte
+    return full.reshape(-1, 4, 32, full.shape[1] // 4, 4).permute(0, 3, 2, 1, 4).reshape(
+        -1, full.shape[1] // 4, 512).contiguous()
+
+
 def check(y, a, b, alpha=1.0):
     """y [R, N] against alpha a b^T of float64 a [R, K], b [N, K]."""
     import torch
@@ -121,6 +132,7 @@ GROUPS = [
     ([300, 0, 57, 129], 5, 333, 672),
     ([257], 0, 1000, 1568),
     ([1, 700], 0, 384, 4128),
+    ([130], 0, 1, 32),
     ([0, 191, 193, 385], 0, 129, 96),
     # few rows, K of whole 128-byte chunks: segments of K side by side in an MMA
     ([1], 0, 2050, 6144),
@@ -452,6 +464,42 @@ def test_two_streams_at_once(cuda_device):
     torch.cuda.synchronize()
     for w, g in zip(want, got):
         assert all(torch.equal(w, y) for y in g)
+
+
+def test_offsets_past_32_bits(cuda_device):
+    """Values of Y, bytes of W and values of X behind 2^32."""
+    import torch
+
+    import candidate_kernel as ck
+
+    n, k, rows = 8192, 128, 530_000  # Y: 4.3e9 values
+    a, b = fp8((rows, k), 1), fp8((2, n, k), 2)
+    one, off = torch.ones(1, device="cuda"), offsets_of([rows - 300, 300])
+    y = ck.fp8_gemm_grouped(a, b, one, off)
+    check(y[-300:], a[-300:].double(), b[1].double())
+    check(y[-600:-300], a[-600:-300].double(), b[0].double())
+    del y
+    torch.cuda.empty_cache()
+    experts, n, k = 40, 8192, 14336  # W: 4.7e9 bytes
+    b = torch.zeros(experts, n, k, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+    b[-1] = fp8((n, k), 3)
+    for c in (2, 100):
+        a = fp8((c, k), 4)
+        off = offsets_of([0] * (experts - 1) + [c])
+        check(ck.fp8_gemm_grouped(a, b, one, off), a.double(), b[-1].double())
+    del b
+    torch.cuda.empty_cache()
+    x = torch.zeros(700_000, 6144, device="cuda", dtype=torch.bfloat16)  # 4.3e9 values
+    x[-200:] = torch.randn(200, 6144, generator=gen(5), device="cuda").bfloat16()
+    codes, scales = ck.mxfp4_quantize(x)
+    want, byte = mx_codes(x[-200:])
+    assert torch.equal(codes[-200:], want)
+    tail = row_scales(scales[-3:], 3 * 128, 192)
+    last = x.shape[0] - (scales.shape[0] - 3) * 128
+    assert torch.equal(tail[last - 200:last], byte)
+    del x
+    back = ck.mxfp4_dequantize(codes, scales)
+    assert torch.equal(back[-200:].double(), mx_values(codes[-200:], scale_block(byte)))
 
 
 @pytest.mark.parametrize("rows,experts,n,k", [(2, 2, 1000, 2048), (40, 4, 300, 1024), (700, 2, 600, 1024)])
