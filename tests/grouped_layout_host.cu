@@ -75,7 +75,10 @@ void check_walk(const tinym::GroupedPlan& g, const std::vector<int>& raw) {
         least = std::min(least, units);
         most = std::max(most, units);
     }
-    if (!p.part_units) expect(most - least <= 1, "equal shares", least, most);
+    const int total = prefix[p.experts] * p.units, share = (total + ctas - 1) / ctas;
+    if (PAIR) expect(most - least <= 1, "equal shares", least, most);
+    else if (!p.part_units) expect(most <= share || (!p.blocked && most <= p.piece_units && 2 * most <= 3 * (share + 1)),
+                                   "shares", most, share);
     else expect(most <= p.part_units * std::max(1, (prefix[p.experts] * p.units + ctas - 1) / ctas),
                 "shares of parts", least, most);
     for (int r = 0; r < p.rows; ++r)
