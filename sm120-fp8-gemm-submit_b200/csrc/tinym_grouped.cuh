@@ -1238,7 +1238,11 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             const int rest = lo + p.rows - hi;
             for (int i = blockIdx.x; i < rest; i += gridDim.x) {
                 __nv_bfloat16* dst = p.y + static_cast<int64_t>(i < lo ? i : hi + i - lo) * p.ldy;
-                for (int n = threadIdx.x - 128; n < p.n; n += 128) dst[n] = __float2bfloat16_rn(0.0f);
+                const int whole = p.wide_y ? p.n / 8 : 0;  // 16-byte stores, then what is left
+                for (int n = threadIdx.x - 128; n < whole; n += 128)
+                    reinterpret_cast<uint4*>(dst)[n] = make_uint4(0u, 0u, 0u, 0u);
+                for (int n = whole * 8 + threadIdx.x - 128; n < p.n; n += 128)
+                    dst[n] = __float2bfloat16_rn(0.0f);
             }
         }
     }

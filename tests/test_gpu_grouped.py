@@ -349,6 +349,31 @@ def test_out_keeps_rows_of_no_group(cuda_device, counts):
     assert torch.equal(one[:, :n], ck.mxfp4_gemm(ac, sa, bc[0], sb[0])) and (one[:, n:] == 7).all()
 
 
+@pytest.mark.parametrize("n", [1024, 1003])
+def test_padded_batch(cuda_device, n):
+    """A row buffer of which a few rows are in use, in the middle: the others
+    are zeros, whatever X holds there."""
+    import torch
+
+    import candidate_kernel as ck
+
+    k, rows = 512, 900
+    off = offsets_of([3, 0, 70], first=400)
+    x = torch.full((rows, k), math.nan, device="cuda")
+    x[400:473] = torch.randn(73, k, generator=gen(1), device="cuda")
+    w = torch.randn(3, n, k, generator=gen(2), device="cuda")
+    a, b = x.to(torch.float8_e4m3fn), w.to(torch.float8_e4m3fn)
+    y = ck.fp8_gemm_grouped(a, b, torch.ones(1, device="cuda"), off)
+    assert not y[:400].any() and not y[473:].any()
+    check(y[400:403], a[400:403].double(), b[0].double())
+    check(y[403:473], a[403:473].double(), b[2].double())
+    (ac, sa), (bc, sb) = ck.mxfp4_quantize(x), ck.mxfp4_quantize(w)
+    y = ck.mxfp4_gemm_grouped(ac, sa, bc, sb, off)
+    assert not y[:400].any() and not y[473:].any()
+    check(y[400:403], mx_values(ac, sa)[400:403], mx_values(bc[0], sb[0]))
+    check(y[403:473], mx_values(ac, sa)[403:473], mx_values(bc[2], sb[2]))
+
+
 @pytest.mark.parametrize("rows", [12, 400])
 def test_offsets_outside_the_rows(cuda_device, rows):
     """Offsets that are not sorted or point outside are clamped, as documented."""
