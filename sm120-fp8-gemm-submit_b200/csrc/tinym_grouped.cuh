@@ -73,6 +73,26 @@ constexpr int kFoldOutBytes = kTileRows * 17 * 4;  // folded: FP32 sums of 128 M
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
+// Read-only loads that stay behind the grid dependency wait: volatile, since the
+// compiler may move a plain read-only load ahead of it.
+__device__ __forceinline__ uint32_t ld_after_wait(const uint32_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint32_t ld_after_wait(const uint8_t* p) {
+    uint32_t v;
+    asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ uint4 ld_after_wait(const uint4* p) {
+    uint4 v;
+    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                 : "l"(p));
+    return v;
+}
+
 // n / d for 0 <= n < 2^31: multiply by ceil(2^(31 + s) / d), 2^s >= d, and shift.
 struct FastDiv {
     uint32_t mul, shift, d;
@@ -631,7 +651,7 @@ __device__ __forceinline__ void grouped_tables(const GroupedParams& p, int32_t* 
     }
     for (int base = 0; base <= p.experts; base += 32) {
         const int i = base + lane;
-        int v = i <= p.experts ? min(max(__ldg(p.offsets + i), 0), p.rows) : 0;
+        int v = i <= p.experts ? min(max(static_cast<int>(ld_after_wait(reinterpret_cast<const uint32_t*>(p.offsets + i))), 0), p.rows) : 0;
         v = max(v, start);
 #pragma unroll
         for (int d = 1; d < 32; d <<= 1) {
@@ -971,10 +991,10 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
 #pragma unroll
                 for (int q = 0; q < kSfPerChunk; ++q) {
                     const int64_t at = static_cast<int64_t>(min(r->block + q, blocks - 1)) * kScaleBlock;
-                    r->w[q] = __ldg(reinterpret_cast<const uint4*>(ws + at));
+                    r->w[q] = ld_after_wait(reinterpret_cast<const uint4*>(ws + at));
 #pragma unroll
                     for (int j = 0; j < 3; ++j)
-                        r->x[q][j] = __ldg(reinterpret_cast<const uint4*>(xs[j] + at));
+                        r->x[q][j] = ld_after_wait(reinterpret_cast<const uint4*>(xs[j] + at));
                 }
             };
             bool more = walk.next(&w);
@@ -1074,14 +1094,14 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                     if constexpr (FOLD) {
 #pragma unroll
                         for (int j = 0; j < 4; ++j)
-                            v[q][j] = __ldg(reinterpret_cast<const uint32_t*>(ws[j] + at));
+                            v[q][j] = ld_after_wait(reinterpret_cast<const uint32_t*>(ws[j] + at));
                     } else {
-                        const uint4 o = __ldg(reinterpret_cast<const uint4*>(ws[0] + at));
+                        const uint4 o = ld_after_wait(reinterpret_cast<const uint4*>(ws[0] + at));
                         v[q][0] = o.x, v[q][1] = o.y, v[q][2] = o.z, v[q][3] = o.w;
                     }
 #pragma unroll
                     for (int j = 0; j < 2; ++j)
-                        v[q][4 + j] = __ldg(reinterpret_cast<const uint32_t*>(xs[j] + at));
+                        v[q][4 + j] = ld_after_wait(reinterpret_cast<const uint32_t*>(xs[j] + at));
                 }
             };
             fetch();

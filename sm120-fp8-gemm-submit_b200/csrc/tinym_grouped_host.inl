@@ -245,28 +245,25 @@ int mx_launch(bool quantize, const void* wide, int32_t dtype, const void* codes,
         (p.runs + kWarps - 1) / kWarps,
         quantize ? (p.pad_words + tinym::kMxThreads - 1) / tinym::kMxThreads : 1);
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(want, int64_t(di->sm_count) * 8));
-    auto s = static_cast<cudaStream_t>(stream);
-    const uint8_t* c = static_cast<const uint8_t*>(codes);
-    const uint8_t* sc = static_cast<const uint8_t*>(scales);
-    if (quantize) {
-        uint8_t* co = const_cast<uint8_t*>(c);
-        uint8_t* so = const_cast<uint8_t*>(sc);
-        if (dtype == TINYM_ACT_BF16)
-            tinym::tinym_mxfp4_quantize_kernel<__nv_bfloat16><<<grid, tinym::kMxThreads, 0, s>>>(
-                static_cast<const __nv_bfloat16*>(wide), co, so, p);
-        else
-            tinym::tinym_mxfp4_quantize_kernel<float><<<grid, tinym::kMxThreads, 0, s>>>(
-                static_cast<const float*>(wide), co, so, p);
-    } else {
-        void* o = const_cast<void*>(wide);
-        if (dtype == TINYM_ACT_BF16)
-            tinym::tinym_mxfp4_dequantize_kernel<__nv_bfloat16><<<grid, tinym::kMxThreads, 0, s>>>(
-                c, sc, static_cast<__nv_bfloat16*>(o), p);
-        else
-            tinym::tinym_mxfp4_dequantize_kernel<float><<<grid, tinym::kMxThreads, 0, s>>>(
-                c, sc, static_cast<float*>(o), p);
-    }
-    e = cudaGetLastError();
+    static const void* const kFn[2][2] = {
+        {reinterpret_cast<const void*>(&tinym::tinym_mxfp4_dequantize_kernel<float>),
+         reinterpret_cast<const void*>(&tinym::tinym_mxfp4_dequantize_kernel<__nv_bfloat16>)},
+        {reinterpret_cast<const void*>(&tinym::tinym_mxfp4_quantize_kernel<float>),
+         reinterpret_cast<const void*>(&tinym::tinym_mxfp4_quantize_kernel<__nv_bfloat16>)}};
+    cudaLaunchConfig_t cfg{};
+    cudaLaunchAttribute attr{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(tinym::kMxThreads);
+    cfg.stream = static_cast<cudaStream_t>(stream);
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = kUsePdl ? 1 : 0;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    // quantise: x, codes, scales; dequantise: codes, scales, y
+    void* q_args[4] = {&wide, &codes, &scales, &p};
+    void* d_args[4] = {&codes, &scales, &wide, &p};
+    e = cudaLaunchKernelExC(&cfg, kFn[quantize ? 1 : 0][dtype == TINYM_ACT_BF16 ? 1 : 0],
+                            quantize ? q_args : d_args);
     if (e != cudaSuccess) return cuda_fail(e, "MXFP4 kernel launch");
     return TINYM_OK;
 }

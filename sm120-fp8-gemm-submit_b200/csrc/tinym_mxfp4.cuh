@@ -55,7 +55,7 @@ struct MxVec;
 template <>
 struct MxVec<__nv_bfloat16> {
     uint4 v;
-    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) { v = ld_after_wait(reinterpret_cast<const uint4*>(p)); }
     __device__ __forceinline__ void zero() { v = make_uint4(0u, 0u, 0u, 0u); }
     // magnitudes compare as integers; NaN above infinity above all
     __device__ __forceinline__ uint32_t top() const {
@@ -69,8 +69,8 @@ template <>
 struct MxVec<float> {
     uint4 a, b;
     __device__ __forceinline__ void load(const float* p) {
-        a = __ldg(reinterpret_cast<const uint4*>(p));
-        b = __ldg(reinterpret_cast<const uint4*>(p) + 1);
+        a = ld_after_wait(reinterpret_cast<const uint4*>(p));
+        b = ld_after_wait(reinterpret_cast<const uint4*>(p) + 1);
     }
     __device__ __forceinline__ void zero() { a = b = make_uint4(0u, 0u, 0u, 0u); }
     __device__ __forceinline__ uint32_t top() const {
@@ -90,6 +90,8 @@ __global__ void __launch_bounds__(kMxThreads)
     tinym_mxfp4_quantize_kernel(const T* __restrict__ x, uint8_t* __restrict__ codes,
                                 uint8_t* __restrict__ scales, const MxParams p) {
     constexpr int kSteps = kMxSteps<T>;
+    grid_dependency_wait();  // launched while the kernel before may still run
+    grid_launch_dependents();
     const int lane = threadIdx.x & 31;
     const uint32_t warps = gridDim.x * (kMxThreads / 32);
     for (uint32_t run = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); run < p.runs; run += warps) {
@@ -160,6 +162,8 @@ __global__ void __launch_bounds__(kMxThreads)
                                   const uint8_t* __restrict__ scales, T* __restrict__ y,
                                   const MxParams p) {
     constexpr int kSteps = kMxSteps<T>;
+    grid_dependency_wait();  // launched while the kernel before may still run
+    grid_launch_dependents();
     const int lane = threadIdx.x & 31;
     const uint32_t warps = gridDim.x * (kMxThreads / 32);
     for (uint32_t run = blockIdx.x * (kMxThreads / 32) + (threadIdx.x >> 5); run < p.runs; run += warps) {
@@ -173,8 +177,8 @@ __global__ void __launch_bounds__(kMxThreads)
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
             const bool in = col + u * 256 < p.k;
-            c[u] = in ? __ldg(reinterpret_cast<const uint32_t*>(codes + (at + u * 256) / 2)) : 0u;
-            s[u] = in ? __ldg(byte + u * 2 * kScaleBlock) : 0u;
+            c[u] = in ? ld_after_wait(reinterpret_cast<const uint32_t*>(codes + (at + u * 256) / 2)) : 0u;
+            s[u] = in ? ld_after_wait(byte + u * 2 * kScaleBlock) : 0u;
         }
 #pragma unroll
         for (int u = 0; u < kSteps; ++u) {
