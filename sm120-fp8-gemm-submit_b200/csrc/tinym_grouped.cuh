@@ -743,11 +743,17 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         fence_mbar_init();
         fence_proxy_async_smem();
     }
-    if (warp == 1) Ops::alloc(smem_u32(tmem_slot), p.tmem_cols);
     // Everything above overlaps the previous kernel's tail (programmatic
     // dependent launch); no global memory is read before it has completed.
     grid_dependency_wait();
-    grid_launch_dependents();
+    if (warp == 1) {
+        // Tensor memory is taken behind that wait, and the next kernel may
+        // start only when it has been: a CTA that held some while it waits
+        // for the grid before, beside one of that grid that waits for some,
+        // would wait for good.
+        Ops::alloc(smem_u32(tmem_slot), p.tmem_cols);
+        grid_launch_dependents();
+    }
     if (warp == 0) grouped_tables(p, off, prefix, lane);
     uint32_t tmem = 0u;
     if constexpr (PAIR) {

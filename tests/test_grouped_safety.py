@@ -1,0 +1,34 @@
+"""CPU: rules of the grouped kernel whose breach could hang the GPU or race on
+its memory, checked on the source and on the plans.  No GPU is touched."""
+
+from __future__ import annotations
+
+import re
+
+from test_kernel_layout import CSRC
+
+
+def _code(name):
+    """A source file without its comments."""
+    text = (CSRC / name).read_text()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    return re.sub(r"//[^\n]*", "", text)
+
+
+def _kernel():
+    code = _code("tinym_grouped.cuh")
+    return code[code.index("tinym_grouped_kernel("):]
+
+
+def test_tensor_memory_is_allocated_between_wait_and_trigger():
+    """No CTA holds tensor memory while it waits for the grid before, and no
+    dependent CTA can come to an SM before this grid's CTA there has its own:
+    else each could hold what the other waits for."""
+    kernel = _kernel()
+    wait, alloc, trigger = (kernel.index(s) for s in
+                            ("grid_dependency_wait()", "Ops::alloc(", "grid_launch_dependents()"))
+    assert wait < alloc < trigger
+    assert kernel.count("Ops::alloc(") == kernel.count("grid_launch_dependents()") == 1
+    # by the allocating warp alone: `if (warp == 1) { alloc; trigger }`
+    between = kernel[kernel.rindex("if (warp == 1) {", 0, alloc):trigger]
+    assert "}" not in between
