@@ -429,6 +429,10 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     while (stages >= 2 && bytes_for(stages) > smem_limit) --stages;
     if (stages < 2) return "no two stages fit";
     g.smem = bytes_for(stages);
+    // A pair wants 512 columns of tensor memory in two SMs at once.  Its CTAs
+    // take all shared memory and so are alone on their SMs: nothing else holds
+    // columns there, where two kernels with one SM each would wait for good.
+    if (g.pair) g.smem = smem_limit;
     *out = g;
     return nullptr;
 }

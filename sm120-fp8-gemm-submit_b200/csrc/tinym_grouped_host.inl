@@ -173,7 +173,8 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
     grouped_config(g, stream, &cfg, attrs);
     if (g.pair) {
         // Pairs need two SMs of one cluster: a persistent grid of more pairs
-        // than are resident at once would run its last ones alone.
+        // than are resident at once would run its last ones alone.  One count
+        // serves every call: a pair's CTAs always take all shared memory.
         int pairs = g_grouped_pairs[dev].load(std::memory_order_relaxed);
         if (!pairs) {
             e = cudaOccupancyMaxActiveClusters(&pairs, fn, &cfg);

@@ -4,8 +4,11 @@ its memory, checked on the source and on the plans.  No GPU is touched."""
 from __future__ import annotations
 
 import re
+import subprocess
 
-from test_kernel_layout import CSRC
+import pytest
+
+from test_kernel_layout import CSRC, ROOT, _nvcc
 
 
 def _code(name):
@@ -32,3 +35,18 @@ def test_tensor_memory_is_allocated_between_wait_and_trigger():
     # by the allocating warp alone: `if (warp == 1) { alloc; trigger }`
     between = kernel[kernel.rindex("if (warp == 1) {", 0, alloc):trigger]
     assert "}" not in between
+
+
+def test_plans(tmp_path):
+    nvcc = _nvcc()
+    if nvcc is None:
+        pytest.skip("nvcc not found")
+    exe = tmp_path / "grouped_safety_host"
+    build = subprocess.run(
+        [nvcc, "-std=c++17", "-O1", "-gencode", "arch=compute_100a,code=sm_100a", "-I", str(CSRC),
+         "-I", str(ROOT / "include"), str(ROOT / "tests" / "grouped_safety_host.cu"), "-o", str(exe)],
+        capture_output=True, text=True, timeout=600)
+    assert build.returncode == 0, build.stderr[-4000:]
+    run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert run.returncode == 0, run.stdout[-4000:]
+    assert run.stdout.startswith("grouped safety checks ok ("), run.stdout
