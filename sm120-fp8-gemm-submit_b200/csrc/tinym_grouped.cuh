@@ -517,14 +517,28 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         : "memory");
 }
 
-// Arrive on a barrier of another CTA of the cluster (a cluster address), with
-// the default release at CTA scope: what it announces (bulk copies that have
-// landed in this CTA's shared memory, scales behind a proxy fence, tensor
-// memory that has been read) is complete in this SM when it is sent, and only
-// tensor-core operations that the other CTA issues later depend on it.  A
-// release at cluster scope took ~1,000 cycles here, twice a stage's MMAs.
+// Arrive on a barrier of another CTA of the cluster (a cluster address): what
+// this CTA's threads stored in its shared memory, up to here, is ordered at
+// cluster scope before what the other CTA does behind its wait.  Nothing else
+// is announced this way, so the release is restricted to shared memory: one of
+// all memory takes more than two stages' MMAs (MXFP4, 4096 x 16384 x 5120:
+// 253 us).
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t cluster_bar) {
-    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+    asm volatile(
+        "fence.release.sync_restrict::shared::cta.cluster;\n\t"
+        "mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar)
+        : "memory");
+}
+
+// 3-D tiled copy of one CTA of a pair to its own shared memory; its bytes are
+// completed on `bar`, a barrier of either CTA (a cluster address).
+__device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar,
+                                                 int32_t c0, int32_t c1, int32_t c2, uint64_t policy) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.cta_group::2"
+        ".L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;" ::"r"(dst),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy)
+        : "memory");
 }
 
 // Bounded wait of a whole warp: no lane diverges and the outcome is uniform.
@@ -733,9 +747,9 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     }
     if (threadIdx.x == 0) {
         for (int s = 0; s < stages; ++s) {
-            // full: the producer's expect_tx (and the bytes), the scales, and
-            // at CTA 0 of a pair the stage of CTA 1
-            mbar_init(full_bar(s), 1 + (FP4 ? 1 : 0) + (PAIR && rank == 0 ? 1 : 0));
+            // full: the producer's expect_tx (and the bytes), the scales.  A
+            // pair uses that of CTA 0, for both CTAs' bytes and scales.
+            mbar_init(full_bar(s), 1 + (FP4 ? kCtas : 0));
             mbar_init(empty_bar(s), 1);
         }
         for (int b = 0; b < 2; ++b) {
@@ -815,13 +829,13 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                 const uint32_t bar = full_bar(s);
                 const int c0 = i * kChunks;
                 if (elect_one()) {
-                    // Only CTA 0 sees the MMAs retire: it passes the free slot on.
-                    if (PAIR && rank == 0 && issued >= stages)
-                        mbar_arrive_remote(at_rank(empty_bar(s), 1));
                     if constexpr (PAIR) {
-                        mbar_expect_tx(bar, (kTileRows + x_rows) * kBlockK);
-                        tma_load_3d(wd, mw, bar, c0 * kBlockK, w_row, w.e, pol_w);
-                        tma_load_3d(xd, mx, bar, c0 * kBlockK, x_row, 0, pol_x);
+                        // Both CTAs' copies complete on CTA 0's barrier, which
+                        // may get CTA 1's bytes ahead of its own expect_tx.
+                        const uint32_t pair_bar = at_rank(bar, 0);
+                        if (rank == 0) mbar_expect_tx(bar, kCtas * (kTileRows + x_rows) * kBlockK);
+                        tma_load_3d_pair(wd, mw, pair_bar, c0 * kBlockK, w_row, w.e, pol_w);
+                        tma_load_3d_pair(xd, mx, pair_bar, c0 * kBlockK, x_row, 0, pol_x);
                     } else if constexpr (FOLD) {
                         mbar_expect_tx(bar, segs * (w_rows + x_rows) * kChunks * kBlockK);
                         tma_load_5d(wd, mw, bar, 0, w_row, 0, c0, w.e, pol_w);
@@ -852,6 +866,15 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                 }
             }
         }
+        // CTA 0's commits arrive at CTA 1's slots: it stays until the last has.
+        if (rank)
+            for (int j = 0; ok && j < stages; ++j) {
+                ok = warp_wait<PAIR>(empty_bar(s), ph, guard, kErrProducerWait);
+                if (++s == stages) {
+                    s = 0;
+                    ph ^= 1u;
+                }
+            }
         if (lane == 0 && *abort_flag) {
             // Wait (bounded) for the copies still in flight before shared
             // memory is released; a stage that lacks another arrival runs
@@ -925,8 +948,12 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                                 }
                             }
                         }
-                        Ops::commit(empty_bar(s));
-                        if (i == nkb - 1) Ops::commit(acc_full(b));
+                        // both CTAs of a pair wait for the MMAs
+#pragma unroll
+                        for (int r = 0; r < kCtas; ++r) {
+                            Ops::commit(r ? at_rank(empty_bar(s), r) : empty_bar(s));
+                            if (i == nkb - 1) Ops::commit(r ? at_rank(acc_full(b), r) : acc_full(b));
+                        }
                     }
                     __syncwarp();
                     if (i == 0) walk.ahead();
@@ -944,23 +971,6 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                 __syncwarp();
                 if (lane == 0) mbar_drain(drain_bar, 0, guard, kErrDrain);
                 __syncwarp();
-            }
-        } else {
-            // CTA 1: pass the arrival of its data and scales on to CTA 0.
-            int s = 0;
-            uint32_t ph = 0u;
-            bool ok = true;
-            while (ok && walk.next(&w)) {
-                for (int i = 0; i < nkb; ++i) {
-                    if (!(ok = warp_wait(full_bar(s), ph, guard, kErrMmaWait))) break;
-                    if (elect_one()) mbar_arrive_remote(at_rank(full_bar(s), 0));
-                    __syncwarp();
-                    if (i == 0) walk.ahead();
-                    if (++s == stages) {
-                        s = 0;
-                        ph ^= 1u;
-                    }
-                }
             }
         }
     } else if (warp < 4) {
@@ -1037,7 +1047,10 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
-                if (elect_one()) mbar_arrive(full_bar(s));
+                if (elect_one()) {
+                    if (rank) mbar_arrive_remote(at_rank(full_bar(s), 0));
+                    else mbar_arrive(full_bar(s));
+                }
                 __syncwarp();
                 if ((s += 2) >= stages) {
                     s -= stages;
@@ -1151,9 +1164,6 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             bool ready = warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait);
             if constexpr (FOLD) ready = epilogue_all(ready);  // the warps meet below: all or none
             if (!ready) break;
-            // The MMAs' commit reaches CTA 0 alone: pass it on.
-            if (PAIR && rank == 0 && warp == 4 && lane == 0)
-                mbar_arrive_remote(at_rank(acc_full(b), 1));
             tc_fence_after_sync();
             const uint32_t taddr = tmem + b * p.acc_cols + (static_cast<uint32_t>(q * 32) << 16);
             __nv_bfloat16* row0 = p.y + static_cast<int64_t>(w.row0) * p.ldy;

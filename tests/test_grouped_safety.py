@@ -50,3 +50,34 @@ def test_plans(tmp_path):
     run = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
     assert run.returncode == 0, run.stdout[-4000:]
     assert run.stdout.startswith("grouped safety checks ok ("), run.stdout
+
+
+def test_other_ctas_barriers_are_signalled_at_cluster_scope():
+    """What one CTA of a pair wrote is ordered before the other's use of it:
+    a thread that arrives on the other CTA's barrier releases at cluster scope
+    (the arrival itself, or a fence in front of it), and a wait on a barrier
+    that the other CTA signals acquires at it.  Copies and MMAs signal by
+    themselves, at cluster scope by definition."""
+    code = _code("tinym_grouped.cuh")
+    # one spelling of an arrival on another CTA's barrier
+    assert len(re.findall(r"mbarrier\.arrive[\w.:]*shared::cluster", code)) == 1
+    body = code[code.index("void mbar_arrive_remote("):]
+    body = body[:body.index("}")]
+    arrive = re.search(r"mbarrier\.arrive\.(\w+)\.cluster\.shared::cluster", body)
+    assert arrive
+    if arrive.group(1) == "relaxed":
+        fence = re.search(r"fence\.(acq_rel|release)[\w.:]*\.cluster;", body)
+        assert fence and fence.start() < arrive.start()
+    else:
+        assert arrive.group(1) == "release"
+    assert "mbarrier.try_wait.parity.acquire.cluster" in code
+    kernel = _kernel()
+    # threads announce their own stores (scales) and what they have read
+    # (accumulators); they pass nothing on
+    announced = re.findall(r"mbar_arrive_remote\(at_rank\((\w+)", kernel)
+    assert sorted(announced) == ["acc_empty", "full_bar"]
+    # every wait acquires at cluster scope in a pair kernel; the one without is
+    # in the scale warps of the others
+    scopes = re.findall(r"warp_wait(<\w+>)?\(", kernel)
+    assert scopes.count("") == 1 and set(scopes) == {"", "<PAIR>", "<true>"}
+    assert "warp_wait(empty_bar(s)" in kernel[kernel.index("if constexpr (FP4 && !PAIR)"):]
