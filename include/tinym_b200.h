@@ -334,6 +334,15 @@ TINYM_API int tinym_selftest_grouped_timeout(const void* x, const void* w, void*
                                              const int32_t* offsets_dev, uint64_t timeout_ns,
                                              void* stream);
 
+/* The same for every kind of operands and of wait: lost = 0 no copies, 1 no
+ * products, 2 products whose end is not announced.  x_scales and w_scales as
+ * in tinym_mxfp4_gemm_grouped, or both NULL (E4M3). */
+TINYM_API int tinym_selftest_grouped_lost(int32_t lost, const void* x, const void* x_scales,
+                                          const void* w, const void* w_scales, void* y, int64_t rows,
+                                          int64_t experts, int64_t n, int64_t k,
+                                          const int32_t* offsets_dev, uint64_t timeout_ns,
+                                          void* stream);
+
 /* ------------------------------------------------------------------------
  * MXFP4: E2M1 elements (0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives), one
  * E8M0 scale byte s (2^(s - 127); 255 = NaN) per 32 consecutive columns.

@@ -144,8 +144,10 @@ struct GroupedMaps {
     CUtensorMap x_tail[4];
 };
 __host__ __device__ constexpr int grouped_x_box(bool pair, int i) { return (pair ? 16 : 8) << i; }
-constexpr uint32_t kGrpNoLoads = 2u;   // self-test: no copy is issued, every wait runs out
 constexpr uint32_t kGrpZeroRest = 1u;  // rows of no group are written as zeros
+// Self-test, so that the waits behind run out: copies, MMAs or the commits of
+// accumulators are not issued.
+constexpr uint32_t kGrpNoLoads = 2u, kGrpNoMma = 4u, kGrpNoCommit = 8u;
 
 constexpr int kBlockUnits = kTileRows / 8;  // 8-row units of a 128-row block
 
@@ -418,7 +420,7 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
         p.w_off = (std::max(p.w_off, front) + 1023u) & ~1023u;
         p.out_off = p.w_off + static_cast<uint32_t>(stages * p.w_stage);
         p.bar_off = p.out_off + (p.fold ? kFoldOutBytes : 4 * kOutBytes);
-        p.tab_off = p.bar_off + 8u * (2 * stages + kGrpBars) + 8u;
+        p.tab_off = p.bar_off + 8u * (2 * stages + kGrpBars) + 16u;
         // The MMA's 128 W rows of the last chunk end inside the allocation.
         const uint32_t read_end = p.w_off + static_cast<uint32_t>(stages * p.w_stage) + kTileRows * kBlockK;
         return std::max(p.tab_off + tables, g.pair ? 0u : read_end) + 1024u;
@@ -721,6 +723,9 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
     const uint32_t drain_bar = bars + 8u * (2 * stages + 4);
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + p.bar_off + 8u * (2 * stages + kGrpBars));
     volatile uint32_t* abort_flag = tmem_slot + 1;
+    // Pair, written by the other CTA: at CTA 0 the stages that CTA 1 has
+    // issued, at CTA 1 whether CTA 0 has given up.
+    volatile uint32_t* peer = tmem_slot + 2;
     int32_t* off = reinterpret_cast<int32_t*>(smem + p.tab_off);
     int32_t* prefix = off + p.experts + 1;
 
@@ -758,6 +763,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         }
         mbar_init(drain_bar, 1);
         *abort_flag = 0u;
+        *peer = 0u;
         fence_mbar_init();
         fence_proxy_async_smem();
     }
@@ -804,12 +810,13 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
         return 32 - __clz((cols - 1) / grouped_x_box(PAIR, 0));  // log2 of the boxes of 8 or 16, rounded up
     };
     const int segs = FOLD ? p.fold : 1;
+    int issued = 0;  // producer: stages
 
     if (warp == 0) {
         // ---------------- TMA producer (the whole warp walks, one lane issues)
         const uint64_t pol_w = PAIR ? l2_policy_evict_normal() : l2_policy_w();
         const uint64_t pol_x = l2_policy_evict_last();
-        int s = 0, issued = 0;
+        int s = 0;
         uint32_t ph = 1u;  // the first pass over the ring does not wait
         bool ok = !(p.flags & kGrpNoLoads);
         while (ok && walk.next(&w)) {
@@ -875,13 +882,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                     ph ^= 1u;
                 }
             }
-        if (lane == 0 && *abort_flag) {
-            // Wait (bounded) for the copies still in flight before shared
-            // memory is released; a stage that lacks another arrival runs
-            // into the limit, long after every copy has landed.
-            for (int j = max(0, issued - stages); j < issued; ++j)
-                if (!mbar_drain(full_bar(j % stages), (j / stages) & 1, guard, kErrDrain)) break;
-        }
+        if (rank && lane == 0) dsmem_st_u32(at_rank(smem_u32(tmem_slot + 2), 0), issued);
     } else if (warp == 1) {
         // ---------------- MMA issuer (the whole warp walks, one lane issues)
         if (rank == 0) {
@@ -890,7 +891,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             const uint64_t db0 = sw128_kmajor_desc(x_ring);
             int s = 0, piece = 0, slot = 0;
             uint32_t ph = 0u;
-            bool ok = true;
+            bool ok = !(p.flags & kGrpNoMma);
             while (ok && walk.next(&w)) {
                 const int b = piece & 1;
                 const uint32_t mma_n = PAIR ? (w.rows + 31) & ~31
@@ -952,7 +953,8 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
 #pragma unroll
                         for (int r = 0; r < kCtas; ++r) {
                             Ops::commit(r ? at_rank(empty_bar(s), r) : empty_bar(s));
-                            if (i == nkb - 1) Ops::commit(r ? at_rank(acc_full(b), r) : acc_full(b));
+                            if (i == nkb - 1 && !(p.flags & kGrpNoCommit))
+                                Ops::commit(r ? at_rank(acc_full(b), r) : acc_full(b));
                         }
                     }
                     __syncwarp();
@@ -964,13 +966,6 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
                     }
                 }
                 ++piece;
-            }
-            if (!ok) {
-                // An abort: wait for every MMA issued so far.
-                if (elect_one()) Ops::commit(drain_bar);
-                __syncwarp();
-                if (lane == 0) mbar_drain(drain_bar, 0, guard, kErrDrain);
-                __syncwarp();
             }
         }
     } else if (warp < 4) {
@@ -1286,17 +1281,42 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             }
         }
     }
-    __syncwarp();
-    tc_fence_before_sync();
-    if constexpr (PAIR) {
-        // Neither CTA leaves while the other may still read its shared memory
-        // or arrive on its barriers.
-        cluster_arrive_release();
-        cluster_wait_acquire();
-    } else {
-        __syncthreads();
+    // The roles meet.  Neither CTA of a pair leaves while the other may still
+    // use its shared memory or arrive on its barriers.
+    auto meet = [&]() {
+        __syncwarp();
+        tc_fence_before_sync();
+        if constexpr (PAIR) {
+            cluster_arrive_release();
+            cluster_wait_acquire();
+        } else {
+            __syncthreads();
+        }
+        tc_fence_after_sync();
+    };
+    if (PAIR && rank == 0 && lane == 0 && *abort_flag) dsmem_st_u32(at_rank(smem_u32(tmem_slot + 2), 1), 1u);
+    meet();
+    // Every accumulator has been stored, so every MMA and copy is over, unless
+    // a wait ran out: then wait (bounded) for what is still in flight before
+    // shared and tensor memory are released.
+    if (PAIR && rank ? *peer != 0 : *abort_flag != 0) {
+        if (warp == 0 && lane == 0 && rank == 0) {
+            // A stage that lacks another arrival runs into the limit, long
+            // after every copy has landed.
+            bool ok = true;
+            for (int j = max(0, issued - stages); ok && j < issued; ++j)
+                ok = mbar_drain(full_bar(j % stages), (j / stages) & 1, guard, kErrDrain);
+            if (PAIR && ok && static_cast<int>(*peer) > issued)  // CTA 1's alone
+                mbar_drain(full_bar(issued % stages), (issued / stages) & 1, guard, kErrDrain);
+        }
+        if (warp == 1 && rank == 0) {
+            if (elect_one()) Ops::commit(drain_bar);
+            __syncwarp();
+            if (lane == 0) mbar_drain(drain_bar, 0, guard, kErrDrain);
+        }
+        if constexpr (PAIR) meet();
+        __syncwarp();
     }
-    tc_fence_after_sync();
     if (warp == 1) Ops::dealloc(tmem, p.tmem_cols);
 }
 

@@ -108,7 +108,7 @@ void grouped_config(const tinym::GroupedPlan& g, void* stream, cudaLaunchConfig_
 int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, const void* w_scales,
                  void* y, int64_t ldy, int64_t rows, int64_t experts, int64_t n, int64_t k_bytes,
                  const int32_t* offsets, const float* alpha, int32_t alpha_count, uint32_t flags,
-                 void* stream, uint64_t timeout_ns = kDefaultTimeoutNs, bool no_loads = false) {
+                 void* stream, uint64_t timeout_ns = kDefaultTimeoutNs, uint32_t selftest = 0u) {
     int dev = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
@@ -152,7 +152,7 @@ int grouped_impl(bool fp4, const void* x, const void* x_scales, const void* w, c
     p.w_scales = static_cast<const uint8_t*>(w_scales);
     if (fp4)
         p.w_scale_stride = (n + 127) / 128 * ((2 * k_bytes + 127) / 128) * tinym::kScaleBlock;
-    p.flags = (flags & TINYM_FLAG_ZERO_REST ? tinym::kGrpZeroRest : 0u) | (no_loads ? tinym::kGrpNoLoads : 0u);
+    p.flags = (flags & TINYM_FLAG_ZERO_REST ? tinym::kGrpZeroRest : 0u) | selftest;
     p.timeout_ns = timeout_ns;
     if ((st = pending_word(di, true, &p.err_host)) != TINYM_OK) return st;
 
@@ -294,7 +294,24 @@ int tinym_selftest_grouped_timeout(const void* x, const void* w, void* y, int64_
     const int st = check_grouped(x, w, y, n, rows, experts, n, k, 16, offsets_dev, nullptr, 0, 0u);
     if (st != TINYM_OK) return st;
     return grouped_impl(false, x, nullptr, w, nullptr, y, n, rows, experts, n, k, offsets_dev, nullptr,
-                        0, 0u, stream, timeout_ns, true);
+                        0, 0u, stream, timeout_ns, tinym::kGrpNoLoads);
+}
+
+int tinym_selftest_grouped_lost(int32_t lost, const void* x, const void* x_scales, const void* w,
+                                const void* w_scales, void* y, int64_t rows, int64_t experts,
+                                int64_t n, int64_t k, const int32_t* offsets_dev,
+                                uint64_t timeout_ns, void* stream) {
+    t_last_error[0] = '\0';
+    static const uint32_t kLost[3] = {tinym::kGrpNoLoads, tinym::kGrpNoMma, tinym::kGrpNoCommit};
+    if (lost < 0 || lost > 2) return fail(TINYM_ERR_INVALID_ARGUMENT, "lost must be 0, 1 or 2 (got %d)", lost);
+    if (timeout_ns == 0 || timeout_ns > 10ull * kDefaultTimeoutNs)
+        return fail(TINYM_ERR_INVALID_ARGUMENT, "timeout_ns must be in 1 .. 1e10");
+    const bool fp4 = x_scales || w_scales;
+    int st = check_grouped(x, w, y, n, rows, experts, n, k, fp4 ? 32 : 16, offsets_dev, nullptr, 0, 0u);
+    if (st == TINYM_OK && fp4) st = check_scales(x_scales, w_scales);
+    if (st != TINYM_OK) return st;
+    return grouped_impl(fp4, x, x_scales, w, w_scales, y, n, rows, experts, n, fp4 ? k / 2 : k, offsets_dev,
+                        nullptr, 0, 0u, stream, timeout_ns, kLost[lost]);
 }
 
 int tinym_mxfp4_gemm_grouped(const void* x, const void* x_scales, const void* w,

@@ -67,6 +67,7 @@ EXPORTED = (
     "tinym_ipc_close",
     "tinym_fp8_gemm_grouped",
     "tinym_selftest_grouped_timeout",
+    "tinym_selftest_grouped_lost",
     "tinym_mxfp4_scale_bytes",
     "tinym_mxfp4_quantize",
     "tinym_mxfp4_dequantize",
@@ -203,6 +204,9 @@ def capi() -> ctypes.CDLL:
             lib.tinym_selftest_grouped_timeout.argtypes = [vp, vp, vp, i64, i64, i64, i64, vp,
                                                            ctypes.c_uint64, vp]
             lib.tinym_selftest_grouped_timeout.restype = ctypes.c_int
+            lib.tinym_selftest_grouped_lost.argtypes = [i32, vp, vp, vp, vp, vp, i64, i64, i64, i64,
+                                                        vp, ctypes.c_uint64, vp]
+            lib.tinym_selftest_grouped_lost.restype = ctypes.c_int
             lib.tinym_mxfp4_scale_bytes.argtypes = [i64, i64, i64, ctypes.POINTER(i64)]
             lib.tinym_mxfp4_scale_bytes.restype = ctypes.c_int
             lib.tinym_mxfp4_quantize.argtypes = [vp, i32, vp, vp, i64, i64, i64, vp]

@@ -81,3 +81,23 @@ def test_other_ctas_barriers_are_signalled_at_cluster_scope():
     scopes = re.findall(r"warp_wait(<\w+>)?\(", kernel)
     assert scopes.count("") == 1 and set(scopes) == {"", "<PAIR>", "<true>"}
     assert "warp_wait(empty_bar(s)" in kernel[kernel.index("if constexpr (FP4 && !PAIR)"):]
+
+
+def test_teardown_decides_on_draining_when_every_role_has_ended():
+    """A wait of any role may run out after the producer or the MMA warp has
+    finished: whether copies and MMAs in flight are waited for is decided
+    behind the barrier at which the roles meet, before tensor memory is freed."""
+    kernel = _kernel()
+    meet = kernel.index("meet();")
+    drains = [m.start() for m in re.finditer(r"mbar_drain\(", kernel)]
+    assert len(drains) >= 2 and all(meet < d < kernel.index("Ops::dealloc(") for d in drains)
+    assert kernel.count("*abort_flag != 0") == 1 and kernel.index("*abort_flag != 0") > meet
+
+
+def test_selftest_refusals():
+    import tinym_b200
+
+    lib, p = tinym_b200.capi(), 1 << 20
+    for lost, xs, ws, ns in [(3, None, None, 1000), (-1, p, p, 1000), (0, p, None, 1000),
+                             (1, None, p, 1000), (2, p, p, 0), (2, p, p, 10 ** 11)]:
+        assert lib.tinym_selftest_grouped_lost(lost, p, xs, p, ws, p, 4, 2, 64, 64, p, ns, None) == 1
