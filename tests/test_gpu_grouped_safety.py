@@ -53,3 +53,39 @@ def test_lost_copies_products_and_commits_are_reported(cuda_device, rows, expert
     assert torch.equal(call(), want)
     assert t.device_status(clear=True) != 0
     assert t.device_status() == 0 and t.pending_errors() == 0
+
+
+@pytest.mark.parametrize("mx", [False, True])
+def test_short_pair_products_on_three_streams(cuda_device, mx):
+    """Pair kernels of one chunk of K, beside each other and beside split-K
+    clusters and stream kernels: every call ends and is right."""
+    import torch
+
+    import candidate_kernel as ck
+
+    def make(counts, n, k, seed):
+        off = offsets_of(counts)
+        if mx:
+            a, sa = quantized((sum(counts), k), seed)
+            b, sb = quantized((len(counts), n, k), seed + 1)
+            return lambda: ck.mxfp4_gemm_grouped(a, sa, b, sb, off)
+        a, b = fp8((sum(counts), k), seed), fp8((len(counts), n, k), seed + 1)
+        one = torch.ones(1, device="cuda")
+        return lambda: ck.fp8_gemm_grouped(a, b, one, off)
+
+    x, w = fp8((9, 6144), 7), fp8((5120, 6144), 8)
+    alpha = torch.tensor([0.01], device="cuda")
+    lanes = [[make([700, 0, 300], 2000, 96, 1)],
+             [make([130], 5120, 64, 3), make([3, 5], 700, 128, 5)],
+             [lambda: ck.fp8_gemm(x, w, alpha), make([400], 1000, 128, 9)]]
+    want = [[f() for f in lane] for lane in lanes]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in lanes]
+    got = []
+    for _ in range(30):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got.append((i, [f() for f in lanes[i]]))
+    torch.cuda.synchronize()
+    for i, outs in got:
+        assert all(torch.equal(o, w) for o, w in zip(outs, want[i]))
