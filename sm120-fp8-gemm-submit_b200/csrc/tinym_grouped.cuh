@@ -73,21 +73,22 @@ constexpr int kFoldOutBytes = kTileRows * 17 * 4;  // folded: FP32 sums of 128 M
 constexpr int kOutBytes = 32 * 64;   // an epilogue warp's output buffer: 32 X rows x 32 W rows
 constexpr int kSfSlotCols = 32;      // TMEM columns of one chunk's scales (8 for W, 16 for X)
 
-// Read-only loads that stay behind the grid dependency wait: volatile, since the
-// compiler may move a plain read-only load ahead of it.
+// Loads that stay behind the grid dependency wait: volatile, since the compiler
+// may move others ahead of it.  Not .nc: the kernel before may still write
+// what they read while this one already runs, which .nc does not allow.
 __device__ __forceinline__ uint32_t ld_after_wait(const uint32_t* p) {
     uint32_t v;
-    asm volatile("ld.global.nc.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    asm volatile("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
 __device__ __forceinline__ uint32_t ld_after_wait(const uint8_t* p) {
     uint32_t v;
-    asm volatile("ld.global.nc.u8 %0, [%1];" : "=r"(v) : "l"(p));
+    asm volatile("ld.global.u8 %0, [%1];" : "=r"(v) : "l"(p));
     return v;
 }
 __device__ __forceinline__ uint4 ld_after_wait(const uint4* p) {
     uint4 v;
-    asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];"
+    asm volatile("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];"
                  : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
                  : "l"(p));
     return v;
@@ -1154,7 +1155,7 @@ __global__ void __launch_bounds__(kGrpThreads, 1)
             // ahead of the wait, so that its latency is hidden
             float alpha = 1.0f;
             if (p.alpha)
-                asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(alpha) : "l"(p.alpha + w.e * p.alpha_stride) : "memory");
+                asm volatile("ld.global.f32 %0, [%1];" : "=f"(alpha) : "l"(p.alpha + w.e * p.alpha_stride) : "memory");
             walk.ahead();
             bool ready = warp_wait<PAIR>(acc_full(b), (piece >> 1) & 1, guard, kErrEpilogueWait);
             if constexpr (FOLD) ready = epilogue_all(ready);  // the warps meet below: all or none

@@ -192,8 +192,13 @@ __device__ __forceinline__ void epilogue_bar_sync() {
     asm volatile("bar.sync 1, 128;" ::: "memory");
 }
 
+// Behind the dependency wait; not .nc, since the kernel before may write alpha
+// while this one already runs.  Volatile: stays ahead of later waits.
 __device__ __forceinline__ float load_alpha(const TinymParams& p) {
-    return p.alpha_ptr ? __ldg(p.alpha_ptr) : p.alpha;
+    float alpha = p.alpha;
+    if (p.alpha_ptr)
+        asm volatile("ld.global.f32 %0, [%1];" : "=f"(alpha) : "l"(p.alpha_ptr) : "memory");
+    return alpha;
 }
 
 // =====================================================================
@@ -499,10 +504,7 @@ __global__ void __launch_bounds__(kTcThreads, 1)
         grid_dependency_wait();  // alpha may be written by the previous kernel
         // issued early (a volatile load stays ahead of the accumulator wait):
         // its latency hides behind the mainloop
-        if (p.alpha_ptr)
-            asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(alpha) : "l"(p.alpha_ptr) : "memory");
-        else
-            alpha = p.alpha;
+        alpha = load_alpha(p);
         // The cluster barrier (every CTA of the cluster resident, barriers
         // initialised) completes long before the first remote store; waiting
         // here keeps the wait off the output path.

@@ -89,3 +89,43 @@ def test_short_pair_products_on_three_streams(cuda_device, mx):
     torch.cuda.synchronize()
     for i, outs in got:
         assert all(torch.equal(o, w) for o, w in zip(outs, want[i]))
+
+
+@pytest.mark.parametrize("rows", [6, 50, 400, 1000])
+def test_chain_of_kernels_that_start_early(cuda_device, rows):
+    """quantise -> grouped product -> quantise -> product, each launched while
+    the one before ends, captured and replayed on changing X and groups: no
+    step sees what its buffers held before (folded, stream and pair plans)."""
+    import torch
+
+    import candidate_kernel as ck
+
+    k, n = 512, 768
+    g = torch.Generator("cuda").manual_seed(1)
+    x = torch.randn(rows, k, generator=g, device="cuda").bfloat16()
+    w1, s1 = ck.mxfp4_quantize(torch.randn(4, n, k, generator=g, device="cuda"))
+    w2, s2 = ck.mxfp4_quantize(torch.randn(k, n, generator=g, device="cuda"))
+    off = offsets_of([rows - 3, 0, 2, 1])
+
+    def step(wait):
+        wait()
+        a, sa = ck.mxfp4_quantize(x)
+        wait()
+        up = ck.mxfp4_gemm_grouped(a, sa, w1, s1, off)
+        wait()
+        d, sd = ck.mxfp4_quantize(up)
+        wait()
+        return up, d, ck.mxfp4_gemm(d, sd, w2, s2)
+
+    step(torch.cuda.synchronize)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(lambda: None)
+    for i in range(12):
+        x.copy_(torch.randn(rows, k, generator=g, device="cuda") * 2.0 ** (i - 6))
+        off.copy_(offsets_of([i % 4, rows - 3 - i % 4, 0, 3 if i % 2 else 1]))
+        graph.replay()
+        graph.replay()
+        torch.cuda.synchronize()
+        for have, want in zip(got, step(torch.cuda.synchronize)):
+            assert torch.equal(have, want), i

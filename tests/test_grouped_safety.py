@@ -101,3 +101,14 @@ def test_selftest_refusals():
     for lost, xs, ws, ns in [(3, None, None, 1000), (-1, p, p, 1000), (0, p, None, 1000),
                              (1, None, p, 1000), (2, p, p, 0), (2, p, p, 10 ** 11)]:
         assert lib.tinym_selftest_grouped_lost(lost, p, xs, p, ws, p, 4, 2, 64, 64, p, ns, None) == 1
+
+
+def test_kernels_that_start_early_use_no_read_only_loads():
+    """A kernel launched while the one before still writes its inputs may not
+    read them as memory that stays as it is for the kernel's whole run (.nc,
+    __ldg), not even behind the dependency wait."""
+    for name in ("tinym_grouped.cuh", "tinym_mxfp4.cuh", "tinym_kernels.cuh"):
+        code = _code(name)
+        if name == "tinym_kernels.cuh":  # launched after the kernel before has ended
+            code = code[:code.index("tinym_pack_weights_kernel")]
+        assert "global.nc" not in code and "__ldg" not in code, name
