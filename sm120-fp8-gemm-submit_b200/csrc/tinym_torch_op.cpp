@@ -272,6 +272,7 @@ std::tuple<at::Tensor, at::Tensor> mxfp4_quantize(const at::Tensor& x) {
     TORCH_CHECK(k > 0 && k % 32 == 0, "X must have K a positive multiple of 32 (got ", num(k), ")");
     const int64_t batch = d == 3 ? x.size(0) : 1, rb = (rows + 127) / 128, kb = (k + 127) / 128;
     const c10::cuda::CUDAGuard guard(x.device());
+    check_pending();
     const auto bytes = x.options().dtype(at::ScalarType::Byte);
     at::Tensor codes = d == 3 ? at::empty({batch, rows, k / 2}, bytes) : at::empty({rows, k / 2}, bytes);
     at::Tensor scales = d == 3 ? at::empty({batch, rb, kb, 512}, bytes) : at::empty({rb, kb, 512}, bytes);
@@ -287,6 +288,7 @@ at::Tensor mxfp4_dequantize(const at::Tensor& codes, const at::Tensor& scales, a
     TORCH_CHECK(dtype == at::ScalarType::BFloat16 || dtype == at::ScalarType::Float,
                 "dtype must be torch.bfloat16 or torch.float32");
     const c10::cuda::CUDAGuard guard(codes.device());
+    check_pending();
     const auto opt = codes.options().dtype(dtype);
     at::Tensor y = codes.dim() == 3 ? at::empty({s.batch, s.rows, s.k}, opt) : at::empty({s.rows, s.k}, opt);
     if (y.numel() == 0) return y;

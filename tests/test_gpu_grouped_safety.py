@@ -129,3 +129,31 @@ def test_chain_of_kernels_that_start_early(cuda_device, rows):
         torch.cuda.synchronize()
         for have, want in zip(got, step(torch.cuda.synchronize)):
             assert torch.equal(have, want), i
+
+
+@pytest.mark.parametrize("op", ["quantize", "dequantize"])
+def test_conversions_raise_after_a_wait_that_ran_out(cuda_device, op):
+    """The output of a product whose wait ran out is unspecified: quantising or
+    expanding it raises, as every op does, instead of passing it on."""
+    import torch
+
+    import candidate_kernel as ck
+    import tinym_b200 as t
+
+    a, b, off = fp8((4, 512), 1), fp8((2, 64, 512), 2), offsets_of([2, 2])
+    y = ck.fp8_gemm_grouped(a, b, torch.ones(1, device="cuda"), off)
+    codes, scales = ck.mxfp4_quantize(y)
+    call = {"quantize": lambda: ck.mxfp4_quantize(y), "dequantize": lambda: ck.mxfp4_dequantize(codes, scales)}[op]
+    torch.cuda.synchronize()
+    assert t.device_status(clear=True) == 0
+    st = t.capi().tinym_selftest_grouped_lost(0, a.data_ptr(), None, b.data_ptr(), None, y.data_ptr(), 4, 2, 64,
+                                              512, off.data_ptr(), 2_000_000,
+                                              torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    torch.cuda.synchronize()
+    try:
+        with pytest.raises(RuntimeError, match="TINYM_ERR_DEVICE_TIMEOUT"):
+            call()
+        call()
+    finally:
+        t.device_status(clear=True)
