@@ -45,6 +45,14 @@ extern "C" {
 
 #define TINYM_ABI_VERSION 8
 
+/* What has been added since, with nothing that was there changed; a library
+ * without tinym_abi_minor has none of it.
+ *   1: tinym_fp8_gemm_grouped, TINYM_FLAG_ZERO_REST, tinym_mxfp4_scale_bytes,
+ *      tinym_mxfp4_quantize, tinym_mxfp4_dequantize, tinym_mxfp4_gemm,
+ *      tinym_mxfp4_gemm_grouped, tinym_selftest_grouped_timeout,
+ *      tinym_selftest_grouped_lost, tinym_abi_minor */
+#define TINYM_ABI_MINOR 1
+
 /* Exported-symbol marker (the library is built with hidden visibility). */
 #if defined(__GNUC__)
 #define TINYM_API __attribute__((visibility("default")))
@@ -394,6 +402,9 @@ TINYM_API const char* tinym_last_error(void);
 
 /* TINYM_ABI_VERSION of the loaded library. */
 TINYM_API int32_t tinym_abi_version(void);
+
+/* TINYM_ABI_MINOR of the loaded library. */
+TINYM_API int32_t tinym_abi_minor(void);
 
 #ifdef __cplusplus
 } /* extern "C" */

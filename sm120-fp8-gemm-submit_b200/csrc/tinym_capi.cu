@@ -582,6 +582,7 @@ int scratch_address(int dev, void** out) {
 extern "C" {
 
 int32_t tinym_abi_version(void) { return TINYM_ABI_VERSION; }
+int32_t tinym_abi_minor(void) { return TINYM_ABI_MINOR; }
 
 const char* tinym_last_error(void) { return t_last_error; }
 

@@ -76,6 +76,7 @@ EXPORTED = (
     "tinym_status_string",
     "tinym_last_error",
     "tinym_abi_version",
+    "tinym_abi_minor",
 )
 
 
@@ -222,6 +223,8 @@ def capi() -> ctypes.CDLL:
             lib.tinym_status_string.restype = ctypes.c_char_p
             lib.tinym_last_error.argtypes = []
             lib.tinym_last_error.restype = ctypes.c_char_p
+            lib.tinym_abi_minor.argtypes = []
+            lib.tinym_abi_minor.restype = ctypes.c_int32
             lib.tinym_abi_version.argtypes = []
             lib.tinym_abi_version.restype = ctypes.c_int32
             _capi = lib
