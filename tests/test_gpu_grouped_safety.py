@@ -157,3 +157,31 @@ def test_conversions_raise_after_a_wait_that_ran_out(cuda_device, op):
         call()
     finally:
         t.device_status(clear=True)
+
+
+@pytest.mark.parametrize("mx", [False, True])
+@pytest.mark.parametrize("rows,n", [(4, 8192), (40, 2000), (700, 1024)])
+def test_sums_are_kept_in_32_bits(cuda_device, rows, n, mx):
+    """Root mean square error against 64 bits, for the folded, stream and pair
+    kernel.  BF16 rounds a value of [2^e, 2^(e + 1)) to a step of 2^(e - 7), so
+    the rounding's rms is 2^(e - 8) / sqrt(3) <= 2^-8 / sqrt(3) of the value
+    (5 % more for the spread of 30,000 values and more); each of K additions is
+    off by at most 2^-23 of a partial sum, whose rms is at most the whole
+    sum's, and rms values add up: K 2^-23.  An accumulator of 14 bits would be
+    off by ten times as much."""
+    import torch
+
+    import candidate_kernel as ck
+    from test_gpu_grouped import mx_values
+
+    k = 6144
+    if mx:
+        a, sa = quantized((rows, k), 31)
+        b, sb = quantized((n, k), 32)
+        y, want = ck.mxfp4_gemm(a, sa, b, sb), mx_values(a, sa) @ mx_values(b, sb).T
+    else:
+        a, b = fp8((rows, k), 33), fp8((1, n, k), 34)
+        y = ck.fp8_gemm_grouped(a, b, torch.ones(1, device="cuda"), offsets_of([rows]))
+        want = a.double() @ b[0].double().T
+    rms = lambda v: float(v.square().mean().sqrt())
+    assert rms(y.double() - want) <= (1.05 * 2.0 ** -8 / 3 ** 0.5 + k * 2.0 ** -23) * rms(want)
