@@ -27,7 +27,8 @@
  *     CUDA device.  Pointers are device pointers on that device.
  *   - X and W must be 16-byte aligned; Y must be 2-byte aligned.
  *   - Inputs are borrowed; nothing is retained after the call returns
- *     except cached TMA descriptors keyed by (pointer, shape).
+ *     except cached TMA descriptors keyed by (pointer, shape); the grouped
+ *     and MXFP4 products keep none.
  *   - The library allocates no device memory on the call path.  The first
  *     GEMM call on a device allocates one pinned, device-mapped 4-byte host
  *     word (the pending-error word, see tinym_pending_errors); the

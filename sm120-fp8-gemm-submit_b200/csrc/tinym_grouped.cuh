@@ -9,7 +9,7 @@
 // rows.  As in tinym_kernels.cuh the W rows are the MMA's M side (128 TMEM
 // lanes) and X rows its N side, which here is a run-time value in steps of 16
 // up to TN: a group of one row costs an MMA of N = 16, not a padded 128-row
-// tile, and ragged groups waste at most 15 columns of the last tile.
+// tile, and ragged groups waste at most 15 columns of a tile (31 for a pair).
 //
 // The group sizes are read on the device, so nothing about them has to reach
 // the host: a persistent grid of one CTA per SM builds the prefix sum of the
@@ -22,9 +22,9 @@
 //    most 128 rows with the whole of K.  The shares differ by at most one
 //    unit, so every SM streams the same number of bytes whatever the groups
 //    are, with no split of K over CTAs, no workspace and one fixed order of
-//    every sum.  28 experts of 2048 x 5120 E4M3 with 128 rows: 51 us, 5.8 TB/s
-//    (89 % of the measured copy); 60 of 2000 x 4096 MXFP4 with 256 rows: 45 us,
-//    5.8 TB/s.
+//    every sum.  28 experts of 2048 x 5120 E4M3 with 128 rows: 52.5 us, 5.6 TB/s
+//    (86 % of the measured copy); 60 of 2000 x 4096 MXFP4 with 256 rows: 46 us,
+//    5.7 TB/s.
 //  * Folded stream pieces, for so little work that a CTA's share is at most 64
 //    W rows and a tile at most 16 X rows.  An MMA costs ~45 cycles to
 //    issue whether 30 or 128 of its rows are used, and a share takes K / 32
@@ -32,16 +32,21 @@
 //    one MMA: A row a h + r is W row r in segment a, B column b x + t is X row
 //    t in segment b, the S diagonal blocks of the product are the segments'
 //    sums, and the epilogue adds them in order: an S-th of the instructions
-//    (1 x 5120 x 6144: E4M3 11.2 -> 9.2 us, MXFP4 8.4 -> 7.2 us).
+//    (1 x 5120 x 6144: E4M3 11.2 -> 9.2 us, MXFP4 8.4 -> 7.2 us when it came in).
 //  * Pair pieces, for many rows per group, where the time is the
 //    tensor core's: two CTAs (cta_group::2) compute 256 W rows x up to 256 X
 //    rows, 128 bytes of K a stage.  Each loads its 128 W rows and half of the
 //    X rows, so a CTA moves 256 rows of K for 128 x 256 sums where one CTA
 //    alone would move 384: the L2 feeds the SMs at ~42 bytes/clk/SM here,
 //    which held single-CTA 128 x 256 tiles at 1.77 PFLOP/s of E4M3.  Measured:
-//    E4M3 2.65 PFLOP/s in a burst and 2.4 under the power cap (8192 x 5120 x
-//    6144), MXFP4 4.7 and 4.3 (4096 x 16384 x 5120); both sit at 1,000 W with
-//    the SM clock at 1.1 - 1.4 GHz.
+//    E4M3 3.0 PFLOP/s in a burst and 2.4 under the power cap (one matrix, 8192 x
+//    5120 x 6144; the same rows in 8 groups: 2.5 and 2.15), MXFP4 4.9 and 4.2
+//    (4096 x 16384 x 5120); both sit at 1,000 W with the SM clock at 1.1 - 1.4
+//    GHz.
+//    CTA 0 issues the MMAs.  The copies of both CTAs complete on its barriers
+//    and its commits arrive at both CTAs, so no thread passes on what it has
+//    waited for; CTA 1's scales, which threads store, are released to CTA 0 at
+//    cluster scope.
 //
 // MXFP4 scales reach TMEM by tcgen05.cp in blocks of 128 rows x 4 scales
 // (lane i, column j = row 32 j + i), the order in which they lie in memory.
@@ -197,7 +202,8 @@ struct GroupedWalk {
             // over K, and with shares below a piece those CTAs are the last to
             // finish: then every matrix is cut into the same number of parts,
             // a CTA each, unless that makes them half as large again (8
-            // experts of 2048 x 4096 E4M3: 18.8 -> 14.9 us).
+            // experts of 2048 x 4096 E4M3: 18.8 -> 14.9 us, the one shape that
+            // the limit of a half was measured on).
             const int all = pre[p.experts];
             if (!p.blocked && !p.part_units && all > 1 && all <= blocks && share < p.piece_units) {
                 const bool few = all <= kGrpBand;  // worked out by the host: divisions take a while
@@ -331,6 +337,12 @@ inline const char* grouped_plan(bool fp4, int64_t rows, int64_t experts, int64_t
     GroupedParams& p = g.prm;
     const int64_t groups = std::min(experts, rows);
     const int64_t avg = (rows + groups - 1) / groups;
+    // A pair takes 2 - 4 us longer (fewer CTAs, start and end), a stream plan reads
+    // W once more for every 64 rows.  us in a graph, stream at 64 rows, then pair and
+    // stream at 65 and at 256 (K = 6144): E4M3, N = 1024: 11.9, 16.2 and 18.5,
+    // 20.1 and 34.6; N = 5120: 13.2, 16.9 and 24.7, 20.9 and 42.4; MXFP4, N =
+    // 1024: 9.3, 11.5 and 13.8, 11.9 and 23.8; N = 5120: 10.1, 12.3 and 14.1,
+    // 13.8 and 23.9.
     g.pair = avg > 64;
     g.mode = g.pair ? kPair : kStream;
     p.rows = static_cast<int32_t>(rows);

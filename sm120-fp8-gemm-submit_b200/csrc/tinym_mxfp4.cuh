@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(kMxThreads)
             const uint32_t ex = top >> 23;  // biased floor(log2(amax)); 0 below the normal range
             const bool bad = ex == 255u;
             const uint32_t byte = bad ? 255u : max(ex, 2u) - 2u;
-            const float unit = __uint_as_float((254u - byte) << 23);  // 2^-e (0 if bad)
+            const float unit = __uint_as_float((254u - byte) << 23);  // 2^-e (-inf if bad: codes dropped below)
             float f[8];
             v[u].values(f);
             uint32_t packed = 0;
